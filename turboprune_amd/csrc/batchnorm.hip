@@ -80,8 +80,9 @@ TP_DEVICE void store_octet(T* p, const Octet<T>& o) {
 //
 // VALU budget: at 6.3 TB/s each CU must retire a 16B octet every ~6 VALU
 // issue slots, so the inner loop uses explicit bit ops (bf16 -> f32 is a
-// shift / a mask, no v_cvt) and packed f32x2 accumulators (v_pk_add_f32
-// / v_pk_fma_f32): 2 shifts + 1 pk_add + 1 pk_fma per dword (2 elems).
+// shift / a mask, no v_cvt) and f32x2 accumulators: 2 shifts + 2 adds +
+// 2 fmas per dword (2 elems). The build keeps packed fp32 instructions
+// off (setup.py says why), so the pairs are plain scalar arithmetic.
 typedef __attribute__((ext_vector_type(2))) float f32x2;
 
 TP_DEVICE f32x2 bf16pair_to_f32x2(uint32_t d) {
