@@ -6,7 +6,9 @@ The .so lands inside turboprune_amd/ (imported as turboprune_amd._C) so
 it travels to GPU boxes with the source tree.
 """
 
+import glob
 import os
+import zlib
 
 from setuptools import setup
 
@@ -38,7 +40,16 @@ sources = [
     os.path.join(CSRC, "attention.hip"),
     os.path.join(CSRC, "schedulefree.hip"),
     os.path.join(CSRC, "conv_implicit_256.hip"),
+    os.path.join(CSRC, "act8.hip"),
+    os.path.join(CSRC, "rms_norm.hip"),
 ]
+
+# the device objects carry no header dependencies of their own: a macro that
+# names the headers' contents makes a changed header a changed command
+headers = 0
+for path in sorted(glob.glob(os.path.join(CSRC, "*.h"))):
+    with open(path, "rb") as f:
+        headers = zlib.crc32(f.read(), headers)
 
 setup(
     name="turboprune_amd_ext",
@@ -51,7 +62,8 @@ setup(
                 # packed fp32 instructions stay off: some of their forms
                 # have given wrong results on this part
                 "nvcc": ["-O3", "-std=c++17", "-Xclang", "-target-feature",
-                         "-Xclang", "-packed-fp32-ops"],
+                         "-Xclang", "-packed-fp32-ops",
+                         f"-DTP_HEADERS={headers}"],
             },
         )
     ],

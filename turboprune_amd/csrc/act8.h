@@ -1,0 +1,261 @@
+// The 8-bit format of kept activations, and the vector helpers of the
+// kernels that read and write it.
+//
+// A row of C values is cut into blocks of 32. A block holds one power of
+// two 2^e (e8m0: the byte is e + 127) and 32 e4m3 codes; a code c stands
+// for c * 2^e. e is the smallest for which the block's largest finite
+// magnitude is at most 448 * 2^e, within [-126, 126], so nothing
+// saturates and 2^e and 2^-e are both normal floats. NaN and infinities
+// take the code NaN (e4m3 has no infinity) and do not raise e, so one bad
+// value does not cost its neighbours their precision.
+//
+// Why this format: a code has 4 significant bits and the scale is a power
+// of two, so c * 2^e is exact in bf16 (and in fp16 within its range) and
+// matrix instructions on 16-bit operands lose nothing more.
+#pragma once
+
+#include "common.h"
+
+namespace turboprune {
+namespace act8 {
+
+constexpr int kBlk = 32;
+
+typedef __attribute__((ext_vector_type(2))) float f32x2v;
+
+// Rows of any length start at any address that their type allows; the
+// memory pipe takes wide accesses at such addresses, so these types only
+// tell the compiler not to assume more.
+typedef __attribute__((ext_vector_type(4))) uint32_t u32x4;
+typedef u32x4 __attribute__((aligned(4))) u32x4_a4;
+typedef u32x4 __attribute__((aligned(2))) u32x4_a2;
+typedef __attribute__((ext_vector_type(2))) uint32_t u32x2;
+typedef u32x2 __attribute__((aligned(1))) u32x2_a1;
+
+typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2v;
+typedef __attribute__((ext_vector_type(2))) _Float16 f16x2v;
+
+// ---- one 8-element chunk of a row in registers ---------------------------
+template <typename T>
+TP_DEVICE void load8(const T* p, float (&v)[8]);
+template <>
+TP_DEVICE void load8<float>(const float* p, float (&v)[8]) {
+  u32x4 a = *reinterpret_cast<const u32x4_a4*>(p);
+  u32x4 b = *reinterpret_cast<const u32x4_a4*>(p + 4);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    v[i] = __uint_as_float(a[i]);
+    v[i + 4] = __uint_as_float(b[i]);
+  }
+}
+template <>
+TP_DEVICE void load8<__hip_bfloat16>(const __hip_bfloat16* p, float (&v)[8]) {
+  u32x4 d = *reinterpret_cast<const u32x4_a2*>(p);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    v[2 * i] = __uint_as_float(d[i] << 16);
+    v[2 * i + 1] = __uint_as_float(d[i] & 0xffff0000u);
+  }
+}
+template <>
+TP_DEVICE void load8<_Float16>(const _Float16* p, float (&v)[8]) {
+  u32x4 d = *reinterpret_cast<const u32x4_a2*>(p);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    f16x2v e = __builtin_bit_cast(f16x2v, (uint32_t)d[i]);
+    v[2 * i] = (float)e[0];
+    v[2 * i + 1] = (float)e[1];
+  }
+}
+
+// two floats to two packed 16-bit values, each rounded to nearest even
+template <typename T>
+TP_DEVICE uint32_t pack2(float a, float b);
+template <>
+TP_DEVICE uint32_t pack2<__hip_bfloat16>(float a, float b) {
+  bf16x2v r;
+  r[0] = (__bf16)a;
+  r[1] = (__bf16)b;
+  return __builtin_bit_cast(uint32_t, r);
+}
+template <>
+TP_DEVICE uint32_t pack2<_Float16>(float a, float b) {
+  f16x2v r;
+  r[0] = (_Float16)a;
+  r[1] = (_Float16)b;
+  return __builtin_bit_cast(uint32_t, r);
+}
+
+template <typename T>
+TP_DEVICE void store8(T* p, const float (&v)[8]) {
+  if constexpr (sizeof(T) == 4) {
+    u32x4 a, b;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      a[i] = __float_as_uint(v[i]);
+      b[i] = __float_as_uint(v[i + 4]);
+    }
+    *reinterpret_cast<u32x4_a4*>(p) = a;
+    *reinterpret_cast<u32x4_a4*>(p + 4) = b;
+  } else {
+    u32x4 r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = pack2<T>(v[2 * i], v[2 * i + 1]);
+    *reinterpret_cast<u32x4_a2*>(p) = r;
+  }
+}
+
+// n of 8 values of a row (the last chunk of a row has fewer than 8; n <= 0
+// for a lane behind it); the others read as zero and are not written
+template <typename T>
+TP_DEVICE void load8n(const T* p, int n, float (&v)[8]) {
+  if (n >= 8) {
+    load8(p, v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = i < n ? to_float<T>(p[i]) : 0.f;
+  }
+}
+template <typename T>
+TP_DEVICE void store8n(T* p, int n, const float (&v)[8]) {
+  if (n >= 8) {
+    store8(p, v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < n) p[i] = from_float<T>(v[i]);
+  }
+}
+
+// the value that is read back after a store as T
+template <typename T>
+TP_DEVICE float rounded(float v) { return to_float<T>(from_float<T>(v)); }
+template <>
+TP_DEVICE float rounded<float>(float v) { return v; }
+
+// ---- scale and codes -----------------------------------------------------
+// largest over the 4 lanes that hold one block (lanes 4k .. 4k+3)
+TP_DEVICE float quad_max(float v) {
+  int o = __builtin_amdgcn_mov_dpp(__float_as_int(v), 0xB1, 0xf, 0xf, true);
+  v = fmaxf(v, __int_as_float(o));   // quad_perm [1,0,3,2]
+  o = __builtin_amdgcn_mov_dpp(__float_as_int(v), 0x4E, 0xf, 0xf, true);
+  return fmaxf(v, __int_as_float(o));   // quad_perm [2,3,0,1]
+}
+
+TP_DEVICE float finite_abs(float v) {
+  float a = fabsf(v);
+  return a <= 3.402823466e38f ? a : 0.f;   // false for NaN and infinity
+}
+
+// largest finite magnitude of 8 values
+TP_DEVICE float amax8(const float (&v)[8]) {
+  float m = finite_abs(v[0]);
+#pragma unroll
+  for (int i = 1; i < 8; ++i) m = fmaxf(m, finite_abs(v[i]));
+  return m;
+}
+
+// e of the block: amax = m 2^k gives k - 8, one more where m > 1.75
+// (adding 0x1fffff carries into the exponent exactly then)
+TP_DEVICE int block_exp(float amax) {
+  int e = (int)((__float_as_uint(amax) + 0x1fffffu) >> 23) - 135;
+  return max(-126, min(126, e));
+}
+TP_DEVICE float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+
+// 8 codes of values that inv = 2^-e brings to 448 or less; an infinity
+// becomes NaN before the conversion, whose own answer for it is not relied on
+TP_DEVICE uint2 encode8(const float (&v)[8], float inv) {
+  float s[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    float a = v[i] * inv;
+    s[i] = fabsf(a) <= 448.f ? a : __uint_as_float(0x7fc00000u);
+  }
+  int lo = __builtin_amdgcn_cvt_pk_fp8_f32(s[0], s[1], 0, false);
+  lo = __builtin_amdgcn_cvt_pk_fp8_f32(s[2], s[3], lo, true);
+  int hi = __builtin_amdgcn_cvt_pk_fp8_f32(s[4], s[5], 0, false);
+  hi = __builtin_amdgcn_cvt_pk_fp8_f32(s[6], s[7], hi, true);
+  return make_uint2((uint32_t)lo, (uint32_t)hi);
+}
+
+TP_DEVICE void decode8(uint2 c, float scale, float (&v)[8]) {
+  f32x2v a = __builtin_amdgcn_cvt_pk_f32_fp8((int)c.x, false);
+  f32x2v b = __builtin_amdgcn_cvt_pk_f32_fp8((int)c.x, true);
+  f32x2v d = __builtin_amdgcn_cvt_pk_f32_fp8((int)c.y, false);
+  f32x2v e = __builtin_amdgcn_cvt_pk_f32_fp8((int)c.y, true);
+  v[0] = a[0] * scale; v[1] = a[1] * scale;
+  v[2] = b[0] * scale; v[3] = b[1] * scale;
+  v[4] = d[0] * scale; v[5] = d[1] * scale;
+  v[6] = e[0] * scale; v[7] = e[1] * scale;
+}
+
+// a code's value within T's finite range: the largest magnitudes of fp16,
+// bf16 and fp32 round up to a power of two that the type cannot hold
+template <typename T>
+TP_DEVICE float held_in(float v) {
+  constexpr float top = sizeof(T) == 4 ? 3.402823466e38f
+                        : __is_same(T, _Float16) ? 65504.f : 3.3895314e38f;
+  return fabsf(v) > top ? copysignf(top, v) : v;   // NaN stays
+}
+
+TP_DEVICE void store_codes(uint8_t* p, int n, uint2 c) {
+  if (n >= 8) {
+    u32x2 w = {c.x, c.y};
+    *reinterpret_cast<u32x2_a1*>(p) = w;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < n) p[i] = (uint8_t)((i < 4 ? c.x : c.y) >> (8 * (i & 3)));
+  }
+}
+TP_DEVICE uint2 load_codes(const uint8_t* p, int n) {
+  if (n >= 8) {
+    u32x2 w = *reinterpret_cast<const u32x2_a1*>(p);
+    return make_uint2(w[0], w[1]);
+  }
+  uint32_t x = 0, y = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (i < n) x |= (uint32_t)p[i] << (8 * i);
+#pragma unroll
+  for (int i = 4; i < 8; ++i)
+    if (i < n) y |= (uint32_t)p[i] << (8 * (i - 4));
+  return make_uint2(x, y);
+}
+
+// ---- GELU ------------------------------------------------------------------
+// Phi(-t) = exp(-t^2/2) g(t) for t >= 0, with g(t) = u P(u), u = 1/(1+0.315t):
+// g falls smoothly from 1/2 towards 1/(t sqrt(2 pi)), which u P(u) follows.
+// P (degree 7, fitted here to the least largest relative error over [0, 40]
+// with g(0) = 1/2 held, and that exactly in fp32) is within 7.7e-7 of Phi(-t),
+// relative, in fp32. erff would be a two-sided branch of about twice the
+// instructions, and this form shares its exponential with the density that
+// the slope needs.
+TP_DEVICE float normal_tail(float t, float e) {   // e = exp(-t^2/2)
+  float u = __builtin_amdgcn_rcpf(fmaf(0.315f, t, 1.f));
+  float p = 0.03447515890002251f;
+  p = fmaf(p, u, -0.1291443556547165f);
+  p = fmaf(p, u, 0.12537990510463715f);
+  p = fmaf(p, u, 0.005099183414131403f);
+  p = fmaf(p, u, 0.10150090605020523f);
+  p = fmaf(p, u, 0.11120770126581192f);
+  p = fmaf(p, u, 0.12581922113895416f);
+  p = fmaf(p, u, 0.12566225230693817f);
+  return e * (p * u);
+}
+TP_DEVICE float bell_exp(float z) {   // exp(-z^2/2) = 2^(-z^2 / (2 ln 2))
+  return __builtin_amdgcn_exp2f(-0.72134752f * z * z);
+}
+TP_DEVICE float gelu(float z) {
+  float q = normal_tail(fabsf(z), bell_exp(z));
+  return z * (z < 0.f ? q : 1.f - q);
+}
+TP_DEVICE float gelu_slope(float z) {
+  float e = bell_exp(z);
+  float q = normal_tail(fabsf(z), e);
+  return fmaf(z * 0.39894228040143268f, e, z < 0.f ? q : 1.f - q);
+}
+
+}  // namespace act8
+}  // namespace turboprune

@@ -82,6 +82,22 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> bn_fwd(
 std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> bn_bwd(
     const at::Tensor&, const at::Tensor&, const at::Tensor&,
     const at::Tensor&, const at::Tensor&, const at::Tensor&, bool, bool);
+// activations kept in 8 bits (act8.hip)
+std::tuple<at::Tensor, at::Tensor> act8_quantize(const at::Tensor&);
+at::Tensor act8_dequantize(const at::Tensor&, const at::Tensor&,
+                           at::ScalarType);
+std::tuple<at::Tensor, at::Tensor, at::Tensor> gelu_keep8_fwd(
+    const at::Tensor&);
+at::Tensor gelu_keep8_bwd(const at::Tensor&, const at::Tensor&,
+                          const at::Tensor&);
+// root-mean-square norm (rms_norm.hip)
+std::tuple<at::Tensor, c10::optional<at::Tensor>, c10::optional<at::Tensor>,
+           c10::optional<at::Tensor>, c10::optional<at::Tensor>>
+rms_fwd(const at::Tensor&, const c10::optional<at::Tensor>&,
+        const at::Tensor&, double, at::ScalarType, bool, bool);
+std::tuple<at::Tensor, c10::optional<at::Tensor>, at::Tensor> rms_bwd(
+    const at::Tensor&, const c10::optional<at::Tensor>&, const at::Tensor&,
+    const at::Tensor&, const at::Tensor&, at::ScalarType, bool);
 }  // namespace turboprune
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -165,4 +181,16 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         "fused NHWC batchnorm(+relu)(+residual) forward");
   m.def("bn_bwd", &turboprune::bn_bwd,
         "fused NHWC batchnorm(+relu)(+residual) backward");
+  m.def("act8_quantize", &turboprune::act8_quantize,
+        "x -> (e4m3 codes, e8m0 scale per 32 values of a row)");
+  m.def("act8_dequantize", &turboprune::act8_dequantize,
+        "(codes, scales) -> values in the given type");
+  m.def("gelu_keep8_fwd", &turboprune::gelu_keep8_fwd,
+        "exact GELU -> (y, x's codes, x's scales)");
+  m.def("gelu_keep8_bwd", &turboprune::gelu_keep8_bwd,
+        "exact GELU gradient from the kept codes");
+  m.def("rms_fwd", &turboprune::rms_fwd,
+        "residual addition + RMS norm -> (y, h, rstd, codes, scales)");
+  m.def("rms_bwd", &turboprune::rms_bwd,
+        "RMS norm gradient -> (dx, dresidual, dweight)");
 }
