@@ -42,6 +42,7 @@ sources = [
     os.path.join(CSRC, "conv_implicit_256.hip"),
     os.path.join(CSRC, "act8.hip"),
     os.path.join(CSRC, "rms_norm.hip"),
+    os.path.join(CSRC, "linear_act.hip"),
 ]
 
 # the device objects carry no header dependencies of their own: a macro that

@@ -46,6 +46,8 @@ def oracle(x):
         lo = (hi - 1).clamp(min=0)
         dh, dl = E4M3[hi] - u, u - E4M3[lo]
         c = torch.where((dh < dl) | ((dh == dl) & (hi % 2 == 0)), hi, lo)
+        # 256 * 2^120 is no finite float: the code below it is taken
+        c = torch.where((e[:, None] == 120) & (c > 119), 119, c)
         c = torch.where(torch.signbit(v), c + 128, c)
         codes[:, b * 32:(b + 1) * 32] = torch.where(
             fin, c, torch.full_like(c, 127))
@@ -113,8 +115,8 @@ def test_every_16_bit_pattern(dev, dtype):
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_dequantize_every_code(dev, dtype):
     """Every code at every scale, within the type's finite range."""
-    codes = torch.arange(256, dtype=torch.uint8).repeat(253, 1)
-    scales = torch.arange(1, 254, dtype=torch.uint8)[:, None].repeat(1, 8)
+    codes = torch.arange(256, dtype=torch.uint8).repeat(246, 1)
+    scales = torch.arange(1, 247, dtype=torch.uint8)[:, None].repeat(1, 8)
     kept = Act8(codes.view(torch.float8_e4m3fn).to(dev),
                 scales.view(torch.float8_e8m0fnu).to(dev))
     want = codes.view(torch.float8_e4m3fn).double() \

@@ -5,7 +5,8 @@
 // two 2^e (e8m0: the byte is e + 127) and 32 e4m3 codes; a code c stands
 // for c * 2^e. e is the smallest for which the block's largest finite
 // magnitude is at most 448 * 2^e, within [-126, 126], so nothing
-// saturates and 2^e and 2^-e are both normal floats. NaN and infinities
+// saturates (but for the last 6 % below the largest float, whose rounding up
+// would be infinite) and 2^e and 2^-e are both normal floats. NaN and infinities
 // take the code NaN (e4m3 has no infinity) and do not raise e, so one bad
 // value does not cost its neighbours their precision.
 //
@@ -163,14 +164,17 @@ TP_DEVICE int block_exp(float amax) {
 }
 TP_DEVICE float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
-// 8 codes of values that inv = 2^-e brings to 448 or less; an infinity
-// becomes NaN before the conversion, whose own answer for it is not relied on
-TP_DEVICE uint2 encode8(const float (&v)[8], float inv) {
+// 8 codes of values that 2^-e brings to 448 or less. An infinity becomes NaN
+// before the conversion, whose own answer for it is not relied on. At e = 120
+// the codes end at 240, since 256 * 2^120 is no finite float.
+TP_DEVICE uint2 encode8(const float (&v)[8], int e) {
+  float inv = pow2(-e), top = e < 120 ? 448.f : 240.f;
   float s[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     float a = v[i] * inv;
-    s[i] = fabsf(a) <= 448.f ? a : __uint_as_float(0x7fc00000u);
+    s[i] = fabsf(a) <= 448.f ? __builtin_amdgcn_fmed3f(a, -top, top)
+                             : __uint_as_float(0x7fc00000u);
   }
   int lo = __builtin_amdgcn_cvt_pk_fp8_f32(s[0], s[1], 0, false);
   lo = __builtin_amdgcn_cvt_pk_fp8_f32(s[2], s[3], lo, true);
@@ -190,13 +194,14 @@ TP_DEVICE void decode8(uint2 c, float scale, float (&v)[8]) {
   v[6] = e[0] * scale; v[7] = e[1] * scale;
 }
 
-// a code's value within T's finite range: the largest magnitudes of fp16,
-// bf16 and fp32 round up to a power of two that the type cannot hold
+// a code's value within T's finite range: in fp16 the largest magnitudes
+// round up to 65536. NaN stays.
 template <typename T>
 TP_DEVICE float held_in(float v) {
-  constexpr float top = sizeof(T) == 4 ? 3.402823466e38f
-                        : __is_same(T, _Float16) ? 65504.f : 3.3895314e38f;
-  return fabsf(v) > top ? copysignf(top, v) : v;   // NaN stays
+  if constexpr (__is_same(T, _Float16))
+    return fabsf(v) > 65504.f ? copysignf(65504.f, v) : v;
+  else
+    return v;
 }
 
 TP_DEVICE void store_codes(uint8_t* p, int n, uint2 c) {

@@ -63,7 +63,7 @@ __global__ __launch_bounds__(kBlock) void keep_kernel(
     int e = block_exp(quad_max(amax8(v[u])));
     int n = a[u].n;
     if (n <= 0) continue;
-    store_codes(codes + a[u].off, n, encode8(v[u], pow2(-e)));
+    store_codes(codes + a[u].off, n, encode8(v[u], e));
     if ((threadIdx.x & 3) == 0) scales[a[u].blk] = (uint8_t)(e + 127);
     if constexpr (OP == kGelu) {
       float o[8];
@@ -100,7 +100,7 @@ __global__ __launch_bounds__(kBlock) void use_kernel(
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       if constexpr (OP == kGelu)
-        v[i] = g[u][i] * gelu_slope(held_in<float>(v[i]));
+        v[i] = g[u][i] * gelu_slope(v[i]);
       else
         v[i] = held_in<T>(v[i]);
     }

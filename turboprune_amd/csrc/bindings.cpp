@@ -98,6 +98,19 @@ rms_fwd(const at::Tensor&, const c10::optional<at::Tensor>&,
 std::tuple<at::Tensor, c10::optional<at::Tensor>, at::Tensor> rms_bwd(
     const at::Tensor&, const c10::optional<at::Tensor>&, const at::Tensor&,
     const at::Tensor&, const at::Tensor&, at::ScalarType, bool);
+// linear layer with an epilogue (linear_act.hip)
+std::tuple<at::Tensor, c10::optional<at::Tensor>, c10::optional<at::Tensor>>
+linear_act_fwd(const at::Tensor&, const at::Tensor&,
+               const c10::optional<at::Tensor>&,
+               const c10::optional<at::Tensor>&, bool, int64_t);
+std::tuple<c10::optional<at::Tensor>, c10::optional<at::Tensor>,
+           c10::optional<at::Tensor>>
+linear_act_bwd(const at::Tensor&, const c10::optional<at::Tensor>&,
+               const c10::optional<at::Tensor>&,
+               const c10::optional<at::Tensor>&,
+               const c10::optional<at::Tensor>&, const at::Tensor&,
+               const c10::optional<at::Tensor>&, bool,
+               c10::optional<at::ScalarType>, c10::optional<at::ScalarType>);
 }  // namespace turboprune
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -193,4 +206,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         "residual addition + RMS norm -> (y, h, rstd, codes, scales)");
   m.def("rms_bwd", &turboprune::rms_bwd,
         "RMS norm gradient -> (dx, dresidual, dweight)");
+  m.def("linear_act_fwd", &turboprune::linear_act_fwd,
+        "act(x w^T + bias) + residual -> (y, kept z, its scales)");
+  m.def("linear_act_bwd", &turboprune::linear_act_bwd,
+        "gradients of linear_act_fwd -> (dx, dw, dbias)");
 }

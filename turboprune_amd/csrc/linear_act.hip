@@ -1,0 +1,816 @@
+// Masked linear layer with bias, GELU and residual in the product's
+// epilogue, and its gradients, from inputs kept in 8 or 16 bits.
+//
+//   z = x w^T + b,  y = act(z) + r            x (M,K), w (N,K) masked
+//   dz = dy act'(z kept),  dx = dz w,  dw = (dz^T x kept) . mask,
+//   db = column sums of dz,  dr = dy
+//
+// All three products run on one tiled matrix kernel (mm_kernel below).
+
+#include <ATen/ATen.h>
+#include <ATen/hip/HIPContext.h>
+#include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPException.h>
+
+#include "act8.h"
+
+namespace turboprune {
+
+using namespace act8;
+
+std::pair<at::Tensor, at::Tensor> act8_empty(at::IntArrayRef,
+                                             const at::TensorOptions&);
+
+namespace {
+
+typedef __attribute__((ext_vector_type(4))) float f32x4;
+typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
+typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
+typedef __attribute__((ext_vector_type(4))) short s16x4;
+typedef __attribute__((ext_vector_type(8))) short s16x8;
+
+#define TP_LDS __attribute__((address_space(3)))
+
+template <typename T>
+TP_DEVICE f32x4 mma(s16x8 a, s16x8 b, f32x4 c) {
+  if constexpr (__is_same(T, _Float16))
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(
+        __builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0,
+        0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+        __builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0,
+        0);
+}
+
+// What a product writes.
+struct Epi {
+  const void* bias;      // N values, or null
+  const void* res;       // (M,N) residual, or null
+  void* out;             // (M,N)
+  void* z;               // (M,N) kept pre-activation: 16-bit values or codes
+  uint8_t* zscale;       // its scales; null: z holds 16-bit values
+  const float* mask;     // weight gradient: 0/1 per value, or null
+  int bias_f32, res_f32, out_f32, act;
+};
+
+// C[q][p] = sum_k Q P. An operand is a matrix of 16-bit values, with
+// kRowK: row q (or p) holding the values along k, or
+// kColK: row k holding the values along q (or p);
+// kCodes is kColK with 8-bit codes and their scales in place of values.
+enum { kRowK = 0, kColK = 1, kCodes = 2 };
+
+struct Mm {
+  const char *q, *p;     // 16-byte aligned, row distances multiples of 16 B
+  int64_t ldq, ldp;      // row distance in bytes
+  int nq, np;            // rows (kRowK) or columns (kColK) that can be read
+  const uint8_t* pscale; // kCodes: a scale for every 32 codes of a row
+  int M, N, K;           // rows and columns of C, length of the sum
+  int tiles_n, tiles;    // tile grid
+  int ksplit, kper;      // k-tiles of one slab; slab s writes out + s M N
+  Epi e;
+};
+
+constexpr int kBK = 64;
+
+// LDS image of a RowK tile: rows of 64 values (128 B); the 16-byte chunk c of
+// row r sits at c ^ (r & 7), so the 16 rows of a fragment read spread over
+// all banks. Of a ColK tile: 64 rows (along k) of W values; the 32-byte block
+// b of row r sits at b ^ f(r) with f(r) = (r & 3) | (r >> 3 & 1) << 2: the
+// rows that one transposing read touches together then differ in bank.
+template <int W, bool TR>
+struct Tile {
+  static constexpr int kBytes = W * kBK * 2;
+  static constexpr int kRow = TR ? W * 2 : kBK * 2;
+  static constexpr int kLoads = kBytes / 1024;   // wave-wide 16 B loads
+};
+
+typedef __amdgpu_buffer_rsrc_t rsrc_t;
+TP_DEVICE rsrc_t rsrc(const void* p, int64_t bytes) {
+  int n = (int)(bytes < 0x7ffffff0 ? bytes : 0x7ffffff0);
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, n,
+                                           0x00020000);
+}
+constexpr int kOut = 0x7ffffff8;   // an offset that no buffer reaches
+
+// Wave `w` of NW brings its share of a tile into LDS with asynchronous
+// 16-byte loads; what lies outside the matrix arrives as zeros.
+template <int W, bool TR, int NW>
+TP_DEVICE void stage(TP_LDS char* dst, const char* base, int64_t ld,
+                     int first, int count, int kt, int K, int wave,
+                     int lane) {
+  constexpr int PER = Tile<W, TR>::kLoads / NW;
+  static_assert(PER * NW == Tile<W, TR>::kLoads, "loads divide evenly");
+  if constexpr (!TR) {
+    int rows = min(W, count - first);
+    rsrc_t r = rsrc(base + (int64_t)first * ld,
+                    (int64_t)(rows - 1) * ld + (K + 7) / 8 * 16);
+    int c = (lane & 7) ^ (lane >> 3);
+    int off = (lane >> 3) * (int)ld + c * 16;
+    if (kt * kBK + c * 8 >= K) off = kOut;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      int row8 = wave * PER + i;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(
+          r, (TP_LDS void*)(dst + row8 * 1024), 16,
+          off == kOut ? kOut : off + row8 * 8 * (int)ld, kt * kBK * 2, 0, 0);
+    }
+  } else {
+    int k0 = kt * kBK, rows = min(kBK, K - k0);
+    constexpr int RB = W * 2;             // bytes of a row of the tile
+    constexpr int LPR = RB / 16;          // lanes to a row
+    rsrc_t r = rsrc(base + (int64_t)k0 * ld + (int64_t)first * 2,
+                    (int64_t)(rows - 1) * ld + (int64_t)(count - first) * 2);
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      int chunk = (wave * PER + i) * 64 + lane;
+      int row = chunk / LPR, c = chunk % LPR;
+      int f = (row & 3) | ((row >> 3 & 1) << 2);
+      int col = ((c >> 1) ^ f) * 32 + (c & 1) * 16;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(
+          r, (TP_LDS void*)(dst + (wave * PER + i) * 1024), 16,
+          row * (int)ld + col, 0, 0, 0);
+    }
+  }
+}
+
+// Fragment of 16 rows (columns) from `at` and 32 values of k from ks * 32:
+// lane l holds number l % 16, k from (l / 16) * 8.
+template <int W, bool TR>
+TP_DEVICE s16x8 frag(TP_LDS const char* t, int at, int ks, int lane) {
+  int g = lane >> 4, i = lane & 15;
+  if constexpr (!TR) {
+    int row = at + i;
+    int c = (ks * 4 + g) ^ (row & 7);
+    return *reinterpret_cast<TP_LDS const s16x8*>(t + row * 128 + c * 16);
+  } else {
+    int row = ks * 32 + g * 8 + (i >> 2);
+    int f = (i >> 2) | ((g & 1) << 2);
+    TP_LDS const char* a =
+        t + row * (W * 2) + (((at >> 4) ^ f) * 32) + (i & 3) * 8;
+    s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((TP_LDS s16x4*)a);
+    s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+        (TP_LDS s16x4*)(a + 4 * W * 2));
+    return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+  }
+}
+
+// kCodes tiles go through registers: 16 codes of one row, with their scale,
+// become 16 values in two LDS stores. A code times a power of two is exact in
+// bf16; in fp16 it is brought into range first.
+template <typename T, int W, int THREADS>
+struct CodeTile {
+  static constexpr int kPer = W * kBK / 16 / THREADS;
+  u32x4 code[kPer];
+  uint32_t scale[kPer];
+
+  TP_DEVICE void load(const Mm& a, int first, int kt) {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      int at = i * THREADS + threadIdx.x;
+      int row = at / (W / 16), col = first + at % (W / 16) * 16;
+      int64_t k = (int64_t)kt * kBK + row;
+      int n = k < a.K ? a.np - col : 0;
+      const uint8_t* p = (const uint8_t*)a.p + k * a.ldp + col;
+      uint2 lo = load_codes(p, n), hi = load_codes(p + 8, n - 8);
+      code[i] = u32x4{lo.x, lo.y, hi.x, hi.y};
+      scale[i] = n > 0 ? a.pscale[k * ((a.np + 31) / 32) + col / 32] : 0;
+    }
+  }
+
+  TP_DEVICE void store(TP_LDS char* dst) const {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      int at = i * THREADS + threadIdx.x;
+      int row = at / (W / 16), blk = at % (W / 16);
+      int f = (row & 3) | ((row >> 3 & 1) << 2);
+      float sc = __uint_as_float(scale[i] << 23);
+      u32x4 v[2];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if constexpr (__is_same(T, _Float16)) {
+          f32x2v x = __builtin_amdgcn_cvt_pk_f32_fp8((int)code[i][j], false);
+          f32x2v y = __builtin_amdgcn_cvt_pk_f32_fp8((int)code[i][j], true);
+          v[j / 2][j % 2 * 2] =
+              pack2<T>(held_in<T>(x[0] * sc), held_in<T>(x[1] * sc));
+          v[j / 2][j % 2 * 2 + 1] =
+              pack2<T>(held_in<T>(y[0] * sc), held_in<T>(y[1] * sc));
+        } else {
+          v[j / 2][j % 2 * 2] = __builtin_bit_cast(
+              uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(
+                            code[i][j], sc, false));
+          v[j / 2][j % 2 * 2 + 1] = __builtin_bit_cast(
+              uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(
+                            code[i][j], sc, true));
+        }
+      }
+      TP_LDS u32x4* d = (TP_LDS u32x4*)(dst + row * (W * 2) + (blk ^ f) * 32);
+      d[0] = v[0];
+      d[1] = v[1];
+    }
+  }
+};
+
+template <int N>
+TP_DEVICE void wait_and_meet() {
+  // this wave's loads but the newest N have landed and its reads are done;
+  // then every wave's
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N)
+               : "memory");
+}
+
+TP_DEVICE float lanes_max_16_32(float v) {
+  v = fmaxf(v, __shfl_xor(v, 16, kWave));
+  return fmaxf(v, __shfl_xor(v, 32, kWave));
+}
+
+template <typename T>
+TP_DEVICE void epilogue8(const Epi& e, int64_t row, int col, int n, int N,
+                         float (&v)[8]) {
+  // v: 8 neighbouring columns of one row; n of them exist (<= 0: none). The
+  // lanes l, l^16, l^32 and l^48 hold one 32-column block.
+  if (e.bias) {
+    float b[8];
+    if (e.bias_f32)
+      load8n((const float*)e.bias + col, n, b);
+    else
+      load8n((const T*)e.bias + col, n, b);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] += b[i];
+  }
+  if (e.z) {
+    if (e.zscale) {
+      int x = block_exp(lanes_max_16_32(amax8(v)));
+      if (n > 0) {
+        store_codes((uint8_t*)e.z + row * N + col, n, encode8(v, x));
+        if ((col & 31) == 0)
+          e.zscale[row * ((N + 31) / 32) + col / 32] = (uint8_t)(x + 127);
+      }
+    } else {
+      store8n((T*)e.z + row * N + col, n, v);
+    }
+  }
+  if (e.act)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = gelu(v[i]);
+  if (e.res) {
+    float r[8];
+    if (e.res_f32)
+      load8n((const float*)e.res + row * N + col, n, r);
+    else
+      load8n((const T*)e.res + row * N + col, n, r);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] += r[i];
+  }
+  if (e.mask) {
+    float m[8];
+    load8n(e.mask + row * N + col, n, m);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = m[i] != 0.f ? v[i] : 0.f;
+  }
+  if (e.out_f32)
+    store8n((float*)e.out + row * N + col, n, v);
+  else
+    store8n((T*)e.out + row * N + col, n, v);
+}
+
+template <typename T, int BQ, int BP, int WQ, int WP, int QF, int PF,
+          int STAGES>
+__global__ __launch_bounds__(WQ * WP * 64) void mm_kernel(Mm a) {
+  constexpr int NW = WQ * WP;
+  constexpr bool QTR = QF != kRowK, PTR = PF != kRowK;
+  constexpr int QB = Tile<BQ, QTR>::kBytes, PB = Tile<BP, PTR>::kBytes;
+  // asynchronous loads of a wave for one k-tile
+  constexpr int LOADS = (QB + (PF == kCodes ? 0 : PB)) / 1024 / NW;
+  constexpr int MI = BQ / WQ / 16, NI = BP / WP / 16;
+  static_assert(NI % 2 == 0, "columns in pairs of fragments");
+  __shared__ __attribute__((aligned(1024))) char smem[STAGES * (QB + PB)];
+  TP_LDS char* lds = (TP_LDS char*)smem;
+
+  // Workgroups go to the 8 XCDs in turn; each XCD takes a contiguous run of
+  // tiles, so that neighbouring tiles meet in its L2.
+  int wg = blockIdx.x;
+  {
+    int q = a.tiles / 8, r = a.tiles % 8, x = wg % 8;
+    wg = (x < r ? x * (q + 1) : r * (q + 1) + (x - r) * q) + wg / 8;
+  }
+  int m0 = wg / a.tiles_n * BQ, n0 = wg % a.tiles_n * BP;
+  int lane = threadIdx.x & 63;
+  int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  int wq = wave / WP * (BQ / WQ), wp = wave % WP * (BP / WP);
+
+  int kt0 = blockIdx.y * a.kper;
+  int kt1 = min((a.K + kBK - 1) / kBK, kt0 + a.kper);
+
+  auto place = [&](int kt) {
+    return lds + (kt - kt0) % STAGES * (QB + PB);
+  };
+  auto fetch = [&](int kt) {
+    TP_LDS char* b = place(kt);
+    stage<BQ, QTR, NW>(b, a.q, a.ldq, m0, a.nq, kt, a.K, wave, lane);
+    if constexpr (PF != kCodes)
+      stage<BP, PTR, NW>(b + QB, a.p, a.ldp, n0, a.np, kt, a.K, wave, lane);
+  };
+  CodeTile<T, BP, NW * 64> ct;
+
+  f32x4 acc[NI][MI] = {};
+#pragma unroll
+  for (int s = 0; s < STAGES - 1; ++s)
+    if (kt0 + s < kt1) fetch(kt0 + s);
+  if constexpr (PF == kCodes) {
+    if (kt0 < kt1) {
+      ct.load(a, n0, kt0);
+      ct.store(place(kt0) + QB);
+    }
+    if (kt0 + 1 < kt1) ct.load(a, n0, kt0 + 1);
+  }
+  for (int kt = kt0; kt < kt1; ++kt) {
+    // All but the newest STAGES - 2 tiles' loads: tile kt is there. Loads of
+    // codes in flight only make the wait longer than it need be.
+    if (kt + STAGES - 2 < kt1)
+      wait_and_meet<(STAGES - 2) * LOADS>();
+    else
+      wait_and_meet<0>();
+    // every wave has read tile kt - 1, whose place tile kt + STAGES - 1 takes
+    if (kt + STAGES - 1 < kt1) fetch(kt + STAGES - 1);
+    if constexpr (PF == kCodes) {
+      if (kt + 1 < kt1) ct.store(place(kt + 1) + QB);
+      if (kt + 2 < kt1) ct.load(a, n0, kt + 2);
+    }
+    TP_LDS const char* b = place(kt);
+#pragma unroll
+    for (int ks = 0; ks < kBK / 32; ++ks) {
+      s16x8 fq[MI], fp[NI];
+#pragma unroll
+      for (int i = 0; i < MI; ++i)
+        fq[i] = frag<BQ, QTR>(b, wq + i * 16, ks, lane);
+#pragma unroll
+      for (int i = 0; i < NI; ++i)
+        fp[i] = frag<BP, PTR>(b + QB, wp + i * 16, ks, lane);
+#pragma unroll
+      for (int i = 0; i < NI; ++i)
+#pragma unroll
+        for (int j = 0; j < MI; ++j)
+          acc[i][j] = mma<T>(fp[i], fq[j], acc[i][j]);
+    }
+  }
+
+  // Lane l of a fragment holds row l % 16 of C and four columns from
+  // (l / 16) * 4. Swapping 16-lane groups between two neighbouring fragments
+  // leaves every lane with eight neighbouring columns: one 16-byte store.
+  a.e.out = (char*)a.e.out + (int64_t)blockIdx.y * a.M * a.N * 4;
+  int g = lane >> 4;
+#pragma unroll
+  for (int j = 0; j < MI; ++j) {
+    int row = m0 + wq + j * 16 + (lane & 15);
+#pragma unroll
+    for (int i = 0; i < NI; i += 2) {
+      float v[8];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        auto s = __builtin_amdgcn_permlane16_swap(
+            __float_as_uint(acc[i][j][k]), __float_as_uint(acc[i + 1][j][k]),
+            false, false);
+        v[k] = __uint_as_float(s[0]);
+        v[4 + k] = __uint_as_float(s[1]);
+      }
+      int col = n0 + wp + i * 16 + (g & 1) * 16 + (g >> 1) * 8;
+      epilogue8<T>(a.e, row, col, row < a.M ? a.N - col : 0, a.N, v);
+    }
+  }
+}
+
+// sum of the slabs of a split product, masked and rounded
+template <typename T>
+__global__ __launch_bounds__(kBlock) void join_kernel(
+    const float* __restrict__ part, const float* __restrict__ mask,
+    T* __restrict__ out, int64_t n, int slabs) {
+  int64_t i = ((int64_t)blockIdx.x * kBlock + threadIdx.x) * 8;
+  int m = (int)min((int64_t)8, n - i);
+  if (m <= 0) return;
+  float s[8];
+  load8n(part + i, m, s);
+  for (int k = 1; k < slabs; ++k) {
+    float v[8];
+    load8n(part + (int64_t)k * n + i, m, v);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s[j] += v[j];
+  }
+  if (mask) {
+    float v[8];
+    load8n(mask + i, m, v);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s[j] = v[j] != 0.f ? s[j] : 0.f;
+  }
+  store8n(out + i, m, s);
+}
+
+// dz = dy act'(z) and the column sums of dz. 32 threads take 256 neighbouring
+// columns, 8 rows at a time; a block adds its rows in registers and joins them
+// in LDS, so the sums need no atomics and keep their order.
+struct Dz {
+  const void* dy;
+  const void* z;           // 16-bit values or codes; null without act
+  const uint8_t* zscale;
+  void* dz;                // (M, ldz), ldz a multiple of 8; null: only sums
+  float* part;             // (blocks, N); null without a bias
+  int64_t M;
+  int N, ldz;
+};
+template <typename T, typename TG, int CT>
+__global__ __launch_bounds__(kBlock) void dz_kernel(Dz a) {
+  constexpr int RL = kBlock / CT;
+  int c = (blockIdx.x * CT + threadIdx.x % CT) * 8;
+  int n = a.N - c, rl = threadIdx.x / CT;
+  float s[8] = {};
+  if (n > 0) {
+    for (int64_t r = (int64_t)blockIdx.y * RL + rl; r < a.M;
+         r += (int64_t)gridDim.y * RL) {
+      float g[8];
+      load8n((const TG*)a.dy + r * a.N + c, n, g);
+      if (a.z) {
+        float z[8];
+        if (a.zscale) {
+          uint2 q = load_codes((const uint8_t*)a.z + r * a.N + c, n);
+          int e = (int)a.zscale[r * ((a.N + 31) / 32) + c / 32] - 127;
+          decode8(q, pow2(e), z);
+        } else {
+          load8n((const T*)a.z + r * a.N + c, n, z);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) g[i] *= gelu_slope(z[i]);
+      }
+      // the rows end with zeros up to a multiple of 8: g is 0 there
+      if (a.dz) store8((T*)a.dz + r * a.ldz + c, g);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s[i] += g[i];
+    }
+  }
+  if (!a.part) return;
+  __shared__ float sum[RL][CT * 8 + 1];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) sum[rl][threadIdx.x % CT * 8 + i] = s[i];
+  __syncthreads();
+  for (int k = threadIdx.x; k < CT * 8; k += kBlock) {
+    int col = blockIdx.x * CT * 8 + k;
+    if (col >= a.N) continue;
+    float v = 0.f;
+#pragma unroll
+    for (int i = 0; i < RL; ++i) v += sum[i][k];
+    a.part[(int64_t)blockIdx.y * a.N + col] = v;
+  }
+}
+
+template <typename TO>
+__global__ __launch_bounds__(1024) void colsum_kernel(
+    const float* __restrict__ part, TO* __restrict__ out, int n, int C) {
+  __shared__ float sum[16][64];
+  int c = blockIdx.x * 64 + (threadIdx.x & 63), k = threadIdx.x >> 6;
+  float v = 0.f;
+  if (c < C)
+    for (int r = k; r < n; r += 16) v += part[(int64_t)r * C + c];
+  sum[k][threadIdx.x & 63] = v;
+  __syncthreads();
+  if (k == 0 && c < C) {
+#pragma unroll
+    for (int i = 1; i < 16; ++i) v += sum[i][threadIdx.x];
+    out[c] = from_float<TO>(v);
+  }
+}
+
+
+// rows of C values to rows of ldo values (a multiple of 8), zeros behind
+template <typename T>
+__global__ __launch_bounds__(kBlock) void pad_kernel(
+    const T* __restrict__ x, T* __restrict__ out, int64_t chunks, int64_t ldx,
+    int C, int cpr) {
+  int64_t i = (int64_t)blockIdx.x * kBlock + threadIdx.x;
+  if (i >= chunks) return;
+  int64_t row = i / cpr;
+  int c = (int)(i - row * cpr) * 8;
+  float v[8];
+  load8n(x + row * ldx + c, C - c, v);
+  store8(out + (row * cpr) * 8 + c, v);
+}
+
+bool is16(at::ScalarType t) { return t == at::kBFloat16 || t == at::kHalf; }
+
+template <typename F>
+void by16(at::ScalarType t, F&& f) {
+  if (t == at::kBFloat16)
+    f(__hip_bfloat16());
+  else
+    f(_Float16());
+}
+
+hipStream_t current() { return at::hip::getCurrentHIPStream(); }
+
+constexpr int kMaxCols = 1 << 20;   // row offsets of a tile fit 31 bits
+
+// A 2-D matrix that the tiles can load: values of a row together, rows 16
+// bytes aligned and a multiple of 8 values long; a copy where it is not.
+at::Tensor loadable(const at::Tensor& t) {
+  int64_t R = t.size(0), C = t.size(1);
+  bool fits = C % 8 == 0 && (C <= 1 || t.stride(1) == 1) &&
+              (R <= 1 || (t.stride(0) % 8 == 0 && t.stride(0) >= C &&
+                          t.stride(0) <= kMaxCols)) &&
+              reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+  if (fits) return t;
+  auto s = C <= 1 || t.stride(1) == 1 ? t : t.contiguous();
+  int64_t C8 = (C + 7) / 8 * 8;
+  auto out = at::empty({R, C8}, t.options());
+  int64_t chunks = R * C8 / 8;
+  if (chunks)
+    by16(t.scalar_type(), [&](auto z) {
+      using T = decltype(z);
+      pad_kernel<T><<<(unsigned)((chunks + kBlock - 1) / kBlock), kBlock, 0,
+                      current()>>>(
+          (const T*)s.data_ptr(), (T*)out.data_ptr(), chunks, s.stride(0),
+          (int)C, (int)(C8 / 8));
+      C10_HIP_KERNEL_LAUNCH_CHECK();
+    });
+  return out;
+}
+int64_t row_bytes(const at::Tensor& t) {
+  return (t.size(0) <= 1 ? t.size(1) : t.stride(0)) * 2;
+}
+
+template <typename T, int BQ, int BP, int WQ, int WP, int QF, int PF, int ST>
+void launch_mm(Mm a, int slabs) {
+  a.tiles_n = (a.N + BP - 1) / BP;
+  a.tiles = (a.M + BQ - 1) / BQ * a.tiles_n;
+  int kt = (a.K + kBK - 1) / kBK;
+  a.kper = (kt + slabs - 1) / slabs;
+  mm_kernel<T, BQ, BP, WQ, WP, QF, PF, ST>
+      <<<dim3(a.tiles, slabs), WQ * WP * 64, 0, current()>>>(a);
+  C10_HIP_KERNEL_LAUNCH_CHECK();
+}
+
+template <typename T, int QF, int PF>
+void run_mm(const Mm& a, int slabs) {
+  launch_mm<T, 128, 128, 2, 2, QF, PF, 2>(a, slabs);
+}
+
+void check_size(int64_t M, int64_t N, int64_t K) {
+  TORCH_CHECK(M < (int64_t(1) << 31) && N <= kMaxCols && K <= kMaxCols,
+              "linear_act: at most 2^31 rows of ", kMaxCols, " values");
+}
+
+}  // namespace
+
+// (y, z, scales of z). keep: 0 keeps nothing, 1 the pre-activation in 16
+// bits, 2 in 8 bits (only with act).
+std::tuple<at::Tensor, c10::optional<at::Tensor>, c10::optional<at::Tensor>>
+linear_act_fwd(const at::Tensor& x, const at::Tensor& w,
+               const c10::optional<at::Tensor>& bias,
+               const c10::optional<at::Tensor>& residual, bool act,
+               int64_t keep) {
+  TORCH_CHECK(x.is_cuda() && x.dim() == 2 && w.dim() == 2 &&
+                  x.size(1) == w.size(1) && x.size(0) > 0 && x.size(1) > 0 &&
+                  w.size(0) > 0,
+              "linear_act_fwd: x (M,K) and w (N,K) on a GPU, none empty");
+  TORCH_CHECK(is16(x.scalar_type()) && w.scalar_type() == x.scalar_type() &&
+                  w.device() == x.device(),
+              "linear_act_fwd: x and w in bfloat16 or float16, on one device");
+  int64_t M = x.size(0), K = x.size(1), N = w.size(0);
+  check_size(M, N, K);
+  c10::DeviceGuard guard(x.device());
+  auto st = x.scalar_type();
+  Mm a{};
+  at::Tensor b, r, ws;
+  if (bias.has_value()) {
+    TORCH_CHECK(bias->dim() == 1 && bias->size(0) == N &&
+                    bias->device() == x.device() &&
+                    (bias->scalar_type() == st ||
+                     bias->scalar_type() == at::kFloat),
+                "linear_act_fwd: bias of N values in x's type or float32");
+    b = bias->contiguous();
+    a.e.bias = b.data_ptr();
+    a.e.bias_f32 = b.scalar_type() == at::kFloat;
+  }
+  auto ot = st;
+  if (residual.has_value()) {
+    TORCH_CHECK(residual->dim() == 2 && residual->size(0) == M &&
+                    residual->size(1) == N &&
+                    residual->device() == x.device() &&
+                    (residual->scalar_type() == st ||
+                     residual->scalar_type() == at::kFloat),
+                "linear_act_fwd: residual (M,N) in x's type or float32");
+    r = residual->contiguous();
+    a.e.res = r.data_ptr();
+    a.e.res_f32 = r.scalar_type() == at::kFloat;
+    ot = r.scalar_type();
+  }
+  auto xl = loadable(x), wl = loadable(w);
+  auto y = at::empty({M, N}, x.options().dtype(ot));
+  c10::optional<at::Tensor> z, zs;
+  if (act && keep == 1) z = at::empty({M, N}, x.options());
+  if (act && keep == 2) std::tie(z, zs) = act8_empty({M, N}, x.options());
+  if (z) a.e.z = z->data_ptr();
+  if (zs) a.e.zscale = (uint8_t*)zs->data_ptr();
+  a.e.out = y.data_ptr();
+  a.e.out_f32 = ot == at::kFloat;
+  a.e.act = act;
+  a.q = (const char*)xl.data_ptr();
+  a.p = (const char*)wl.data_ptr();
+  a.ldq = row_bytes(xl);
+  a.ldp = row_bytes(wl);
+  a.nq = a.M = (int)M;
+  a.np = a.N = (int)N;
+  a.K = (int)K;
+  by16(st, [&](auto t) { run_mm<decltype(t), kRowK, kRowK>(a, 1); });
+  return {y, z, zs};
+}
+
+// (dx, dw, db), each only where asked for. z: the kept pre-activation (16-bit
+// values, or codes with zscale), null without an activation. xk: the kept
+// input (16-bit values, or codes with xscale). dw has dw_type and the mask
+// applied, db has db_type.
+std::tuple<c10::optional<at::Tensor>, c10::optional<at::Tensor>,
+           c10::optional<at::Tensor>>
+linear_act_bwd(const at::Tensor& dy_in, const c10::optional<at::Tensor>& z,
+               const c10::optional<at::Tensor>& zscale,
+               const c10::optional<at::Tensor>& xkept,
+               const c10::optional<at::Tensor>& xscale, const at::Tensor& w, const c10::optional<at::Tensor>& mask,
+               bool want_dx, c10::optional<at::ScalarType> dw_type,
+               c10::optional<at::ScalarType> db_type) {
+  TORCH_CHECK(dy_in.is_cuda() && dy_in.dim() == 2 && w.dim() == 2 &&
+                  is16(w.scalar_type()) && dy_in.device() == w.device() &&
+                  (xkept.has_value() || !dw_type.has_value()),
+              "linear_act_bwd: dy (M,N), x (M,K) and w (N,K) on a GPU");
+  int64_t M = dy_in.size(0), N = dy_in.size(1), K = w.size(1);
+  auto st = w.scalar_type();
+  TORCH_CHECK(w.size(0) == N && M > 0 && N > 0 && K > 0,
+              "linear_act_bwd: shapes differ from the forward pass");
+  TORCH_CHECK(dy_in.scalar_type() == st || dy_in.scalar_type() == at::kFloat,
+              "linear_act_bwd: dy in w's type or float32");
+  check_size(M, N, K);
+  c10::DeviceGuard guard(w.device());
+  auto dy = dy_in.contiguous();
+  bool g32 = dy.scalar_type() == at::kFloat;
+  int64_t ldz = (N + 7) / 8 * 8;
+  auto opt = w.options();
+  // dy is dz itself where nothing has to be done to it
+  bool same = !z.has_value() && !g32 && N == ldz &&
+              reinterpret_cast<uintptr_t>(dy.data_ptr()) % 16 == 0;
+  bool products = want_dx || dw_type.has_value();
+  at::Tensor dz = same ? dy : at::empty({products ? M : 0, ldz}, opt), part;
+  c10::optional<at::Tensor> dx, dw, db;
+  if ((!same && products) || db_type.has_value()) {
+    Dz d{};
+    d.dy = dy.data_ptr();
+    if (z.has_value()) {
+      TORCH_CHECK(z->sizes() == dy.sizes() && z->is_contiguous() &&
+                      z->device() == w.device() &&
+                      (zscale.has_value()
+                           ? z->scalar_type() == at::kFloat8_e4m3fn &&
+                                 zscale->is_contiguous() &&
+                                 zscale->device() == w.device() &&
+                                 zscale->numel() == M * ((N + 31) / 32)
+                           : z->scalar_type() == st),
+                  "linear_act_bwd: kept pre-activation not of the forward "
+                  "pass");
+      d.z = z->data_ptr();
+      if (zscale.has_value()) d.zscale = (const uint8_t*)zscale->data_ptr();
+    }
+    if (!same && products) d.dz = dz.data_ptr();
+    d.M = M;
+    d.N = (int)N;
+    d.ldz = (int)ldz;
+    bool wide = N > 64;
+    int ct = wide ? 32 : 8, rl = kBlock / ct;
+    int strips = (int)((N + ct * 8 - 1) / (ct * 8));
+    int gy = (int)std::min<int64_t>((M + rl - 1) / rl,
+                                    std::max(1, 1536 / strips));
+    if (db_type.has_value()) {
+      part = at::empty({gy, N}, opt.dtype(at::kFloat));
+      d.part = part.data_ptr<float>();
+    }
+    by16(st, [&](auto t) {
+      using T = decltype(t);
+      dim3 grid(strips, gy);
+      auto s = current();
+      if (wide && g32)
+        dz_kernel<T, float, 32><<<grid, kBlock, 0, s>>>(d);
+      else if (wide)
+        dz_kernel<T, T, 32><<<grid, kBlock, 0, s>>>(d);
+      else if (g32)
+        dz_kernel<T, float, 8><<<grid, kBlock, 0, s>>>(d);
+      else
+        dz_kernel<T, T, 8><<<grid, kBlock, 0, s>>>(d);
+      C10_HIP_KERNEL_LAUNCH_CHECK();
+    });
+    if (db_type.has_value()) {
+      db = at::empty({N}, opt.dtype(*db_type));
+      int grid = (int)((N + 63) / 64);
+      if (*db_type == at::kFloat)
+        colsum_kernel<<<grid, 1024, 0, current()>>>(
+            d.part, db->data_ptr<float>(), gy, (int)N);
+      else
+        by16(*db_type, [&](auto t) {
+          using T = decltype(t);
+          colsum_kernel<<<grid, 1024, 0, current()>>>(
+              d.part, (T*)db->data_ptr(), gy, (int)N);
+        });
+      C10_HIP_KERNEL_LAUNCH_CHECK();
+    }
+  }
+  if (want_dx) {
+    auto wl = loadable(w);
+    dx = at::empty({M, K}, opt);
+    Mm a{};
+    a.q = (const char*)dz.data_ptr();
+    a.ldq = ldz * 2;
+    a.nq = a.M = (int)M;
+    a.p = (const char*)wl.data_ptr();
+    a.ldp = row_bytes(wl);
+    a.np = (int)wl.size(1);
+    a.N = (int)K;
+    a.K = (int)N;
+    a.e.out = dx->data_ptr();
+    by16(st, [&](auto t) { run_mm<decltype(t), kRowK, kColK>(a, 1); });
+  }
+  if (dw_type.has_value()) {
+    dw = at::empty({N, K}, opt.dtype(*dw_type));
+    Mm a{};
+    const at::Tensor& xk = *xkept;
+    TORCH_CHECK(xk.dim() == 2 && xk.size(0) == M && xk.size(1) == K,
+                "linear_act_bwd: kept input not of the forward pass");
+    at::Tensor xl = xk;
+    a.q = (const char*)dz.data_ptr();
+    a.ldq = ldz * 2;
+    a.nq = (int)ldz;
+    a.M = (int)N;
+    a.N = (int)K;
+    a.K = (int)M;
+    at::Tensor xs;
+    if (xscale.has_value()) {
+      TORCH_CHECK(xk.scalar_type() == at::kFloat8_e4m3fn &&
+                      xscale->scalar_type() == at::kFloat8_e8m0fnu &&
+                      xscale->dim() == 2 && xscale->size(0) == M &&
+                      xscale->size(1) == (K + 31) / 32 &&
+                      xk.device() == w.device() &&
+                      xscale->device() == w.device(),
+                  "linear_act_bwd: kept input not of the forward pass");
+      xl = xk.contiguous();
+      xs = xscale->contiguous();
+      a.p = (const char*)xl.data_ptr();
+      a.ldp = K;
+      a.np = (int)K;
+      a.pscale = (const uint8_t*)xs.data_ptr();
+    } else {
+      TORCH_CHECK(xk.scalar_type() == st && xk.device() == w.device(),
+                  "linear_act_bwd: kept input not of the forward pass");
+      xl = loadable(xk);
+      a.p = (const char*)xl.data_ptr();
+      a.ldp = row_bytes(xl);
+      a.np = (int)xl.size(1);
+    }
+    at::Tensor m;
+    if (mask.has_value()) {
+      TORCH_CHECK(mask->numel() == N * K && mask->scalar_type() == at::kFloat,
+                  "linear_act_bwd: float32 mask of w's shape");
+      m = mask->contiguous();
+    }
+    // Few output tiles, a long sum: slabs of it in fp32, joined afterwards.
+    int tiles = (int)((N + 127) / 128 * ((K + 127) / 128));
+    int kts = (int)((M + kBK - 1) / kBK);
+    int slabs = std::max(1, std::min(kts / 4, 512 / tiles));
+    bool join = slabs > 1 || *dw_type != st;
+    at::Tensor part2;
+    if (join) {
+      part2 = at::empty({slabs, N, K}, opt.dtype(at::kFloat));
+      a.e.out = part2.data_ptr();
+      a.e.out_f32 = 1;
+    } else {
+      a.e.out = dw->data_ptr();
+      if (m.defined()) a.e.mask = m.data_ptr<float>();
+    }
+    by16(st, [&](auto t) {
+      using T = decltype(t);
+      if (xscale.has_value())
+        run_mm<T, kColK, kCodes>(a, slabs);
+      else
+        run_mm<T, kColK, kColK>(a, slabs);
+    });
+    if (join) {
+      int64_t n = N * K;
+      unsigned grid = (unsigned)((n + kBlock * 8 - 1) / (kBlock * 8));
+      const float* mp = m.defined() ? m.data_ptr<float>() : nullptr;
+      const float* pp = part2.data_ptr<float>();
+      if (*dw_type == at::kFloat)
+        join_kernel<<<grid, kBlock, 0, current()>>>(
+            pp, mp, dw->data_ptr<float>(), n, slabs);
+      else
+        by16(*dw_type, [&](auto t) {
+          using T = decltype(t);
+          join_kernel<<<grid, kBlock, 0, current()>>>(
+              pp, mp, (T*)dw->data_ptr(), n, slabs);
+        });
+      C10_HIP_KERNEL_LAUNCH_CHECK();
+    }
+  }
+  return {dx, dw, db};
+}
+
+}  // namespace turboprune

@@ -107,7 +107,7 @@ __global__ __launch_bounds__(kBlock) void rms_fwd_kernel(NormFwd p) {
       if (p.codes) {
         int e = block_exp(quad_max(amax8(v[j])));
         if (n > 0) {
-          store_codes(p.codes + row * p.C + c, n, encode8(v[j], pow2(-e)));
+          store_codes(p.codes + row * p.C + c, n, encode8(v[j], e));
           if ((t & 3) == 0)
             p.scales[row * sblk + c / kBlk] = (uint8_t)(e + 127);
         }
@@ -268,7 +268,7 @@ __global__ __launch_bounds__(kBlock) void rms_fwd_long_kernel(NormFwd p) {
       if (p.codes) {
         int e = block_exp(quad_max(amax8(v)));
         if (n > 0) {
-          store_codes(p.codes + row * p.C + c, n, encode8(v, pow2(-e)));
+          store_codes(p.codes + row * p.C + c, n, encode8(v, e));
           if ((threadIdx.x & 3) == 0)
             p.scales[row * sblk + c / kBlk] = (uint8_t)(e + 127);
         }

@@ -21,6 +21,8 @@ import torch
 import torch.nn.functional as F
 
 from turboprune_amd.ops import _backend
+from turboprune_amd.ops import act8
+from turboprune_amd.ops.act8 import Act8
 
 
 def mask_apply(weight: torch.Tensor, mask: torch.Tensor,
@@ -137,6 +139,207 @@ class _MaskedLinearGemm(torch.autograd.Function):
             else:
                 grad_b = gy2.sum(0).to(ctx.bias_dtype)
         return grad_x, grad_w, grad_b
+
+
+ACTS = (None, "gelu")
+
+
+class _MaskedLinearAct(torch.autograd.Function):
+    """One node from the raw weight: product, bias, activation and residual
+    forward; dx, masked dw, db and dresidual backward."""
+
+    @staticmethod
+    def forward(ctx, x, w, weight, mask, bias, residual, act, keep, codes,
+                scales):
+        # the pre-activation is needed by the slope, the input only by dw
+        need = ctx.needs_input_grad
+        need_x, need_z = need[2], need[0] or need[2] or need[4]
+        if keep is not None and codes is None and need_x:
+            codes, scales = act8.quantize_act8(x)
+        y, z, zs = _linear_act_fwd(
+            x, w, bias, residual, act,
+            0 if not need_z else 1 if keep is None else 2)
+        kept = (None, None) if not need_x else \
+            (x, None) if keep is None else (codes, scales)
+        ctx.save_for_backward(w, z, zs, *kept, mask if need_x else None)
+        ctx.weight, ctx.bias = (weight.dtype, weight.shape), \
+            None if bias is None else bias.dtype
+        return y
+
+    @staticmethod
+    def backward(ctx, dy):
+        w, z, zs, xk, xs, mask = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        dx = dw = db = None
+        if need[0] or need[2] or need[4]:
+            dx, dw, db = _linear_act_bwd(
+                dy, z, zs, xk, xs, w, mask, need[0],
+                ctx.weight[0] if need[2] else None,
+                ctx.bias if need[4] else None)
+        if dw is not None:
+            dw = dw.reshape(ctx.weight[1])
+        return (dx, None, dw, None, db, dy if need[5] else None, None, None,
+                None, None)
+
+
+def _linear_act_fwd(x, w, bias, residual, act, keep):
+    if _backend.use_native(x, w):
+        return _backend.extension().linear_act_fwd(
+            x, w, bias, residual, act is not None, keep)
+    from turboprune_amd.ops.norm_act import gelu_plain
+    z = x.float() @ w.float().t()
+    if bias is not None:
+        z = z + bias.float()
+    y = z if act is None else gelu_plain(z)
+    if residual is not None:
+        y = y + residual.float()
+    y = y.to(x.dtype if residual is None else residual.dtype)
+    if act is None or keep == 0:
+        return y, None, None
+    return (y, z.to(x.dtype), None) if keep == 1 else \
+        (y, *act8.quantize_act8(z))
+
+
+def _linear_act_bwd(dy, z, zs, xk, xs, w, mask, want_dx, dw_type, db_type):
+    if _backend.use_native(dy, w):
+        return _backend.extension().linear_act_bwd(
+            dy, z, zs, xk, xs, w, mask, want_dx, dw_type, db_type)
+    from turboprune_amd.ops.norm_act import gelu_slope
+    dz = dy.float()
+    if z is not None:
+        z = z.float() if zs is None else \
+            act8.dequantize_act8(Act8(z, zs), torch.float32)
+        dz = dz * gelu_slope(z)
+    dx = dw = db = None
+    if want_dx:
+        dx = (dz @ w.float()).to(w.dtype)
+    if dw_type is not None:
+        x = xk.float() if xs is None else \
+            act8.dequantize_act8(Act8(xk, xs), torch.float32)
+        dw = dz.t() @ x
+        if mask is not None:
+            dw = torch.where(mask.reshape(dw.shape) != 0, dw,
+                             torch.zeros_like(dw))
+        dw = dw.to(dw_type)
+    if db_type is not None:
+        db = dz.sum(0).to(db_type)
+    return dx, dw, db
+
+
+def masked_linear_act(x: torch.Tensor, weight: torch.Tensor,
+                      mask: Optional[torch.Tensor],
+                      bias: Optional[torch.Tensor] = None,
+                      residual: Optional[torch.Tensor] = None,
+                      act: Optional[str] = None,
+                      cache: Optional[torch.Tensor] = None,
+                      compute_dtype: Optional[torch.dtype] = None,
+                      keep: Optional[str] = None,
+                      kept: Optional[Act8] = None) -> torch.Tensor:
+    """``act(x @ (mask * weight)^T + bias) + residual`` with everything after
+    the product in its epilogue.
+
+    ``x`` is ``(..., K)``, ``weight`` ``(N, K)``; ``mask`` float32 of its shape,
+    or None; ``bias`` ``(N,)``; ``residual`` of the output's shape, in the
+    compute type or float32, which is then the output's type too; ``act`` None
+    or ``"gelu"`` (exact). ``cache`` and ``compute_dtype`` are
+    ``masked_linear``'s: the masked weight in the compute type, and that type
+    where there is no cache. The compute type is bfloat16 or float16 on a GPU
+    (also float32 on the CPU); an ``x`` of another type is cast to it.
+
+    For the backward pass the input and, with an activation, the
+    pre-activation are kept: in the compute type, or with ``keep="e4m3"`` in
+    the 8-bit format of ``ops.act8`` (the gradients are then taken at the
+    values it stands for). ``kept`` is ``x`` already in that format, as
+    ``add_rms_norm`` hands it on. The weight's gradient is masked and has the
+    weight's type.
+    """
+    act8.check_keep(keep)
+    if act not in ACTS:
+        raise ValueError(f"act={act!r}: one of {ACTS}")
+    if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1]:
+        raise ValueError("masked_linear_act: x (..., K) and weight (N, K) "
+                         f"expected, not {tuple(x.shape)} and "
+                         f"{tuple(weight.shape)}")
+    N, K = weight.shape
+    for name, t, shape in (("mask", mask, (N, K)), ("bias", bias, (N,)),
+                           ("cache", cache, (N, K)),
+                           ("residual", residual, x.shape[:-1] + (N,))):
+        if t is not None and t.shape != torch.Size(shape):
+            raise ValueError(f"masked_linear_act: {name} of shape "
+                             f"{tuple(shape)} expected, not {tuple(t.shape)}")
+    for name, t in (("weight", weight), ("mask", mask), ("bias", bias),
+                    ("cache", cache), ("residual", residual)):
+        if t is not None and t.device != x.device:
+            raise ValueError(f"masked_linear_act: {name} on {t.device}, x on "
+                             f"{x.device}")
+    for name, t in (("x", x), ("weight", weight), ("bias", bias)):
+        if t is not None:
+            act8.check_float(name, t)
+    if mask is not None and mask.dtype != torch.float32:
+        raise TypeError(f"masked_linear_act: mask is {mask.dtype}: float32 "
+                        "expected")
+    if cache is not None:
+        w = cache
+    else:
+        ct = compute_dtype or (weight.dtype if weight.dtype != torch.float32
+                               else x.dtype)
+        with torch.no_grad():
+            w = _masked_compute(weight, mask, ct)
+    ct = w.dtype
+    if ct not in (torch.bfloat16, torch.float16) and (
+            x.is_cuda or ct != torch.float32):
+        raise TypeError("masked_linear_act computes in bfloat16 or float16 "
+                        f"on a GPU, not in {ct}: give a cache or a "
+                        "compute_dtype of such a type")
+    if residual is not None and residual.dtype not in (ct, torch.float32):
+        raise TypeError(f"masked_linear_act: residual in {ct} or float32 "
+                        f"expected, not {residual.dtype}")
+    if kept is not None:
+        if keep is None:
+            raise ValueError("masked_linear_act: kept needs keep='e4m3'")
+        act8.check_act8(kept, like=x)
+    if x.dtype != ct:
+        x = x.to(ct)
+    if bias is not None and bias.dtype not in (ct, torch.float32):
+        bias = bias.to(ct)
+    lead = x.shape[:-1]
+    x2 = x if x.dim() == 2 else x.reshape(-1, K)
+    r2 = residual if residual is None or residual.dim() == 2 else \
+        residual.reshape(-1, N)
+    if x2.numel() == 0 or N == 0:
+        y = _linear_of_nothing(x2, weight, bias, r2, ct)
+    elif torch.is_grad_enabled() and any(
+            t is not None and t.requires_grad
+            for t in (x, weight, bias, residual)):
+        codes, scales = (None, None) if kept is None else \
+            (kept.codes.reshape(x2.shape), kept.scales.reshape(
+                x2.shape[0], -1))
+        y = _MaskedLinearAct.apply(x2, w, weight, mask, bias, r2, act, keep,
+                                   codes, scales)
+    else:
+        y = _linear_act_fwd(x2, w, bias, r2, act, 0)[0]
+    return y if x.dim() == 2 else y.reshape(lead + (N,))
+
+
+def _masked_compute(weight, mask, dtype):
+    if mask is None:
+        return weight.to(dtype)
+    if weight.dtype == torch.float32 and dtype in (torch.float32,
+                                                   torch.bfloat16):
+        return mask_apply(weight, mask, dtype)
+    return torch.where(mask != 0, weight, torch.zeros_like(weight)).to(dtype)
+
+
+def _linear_of_nothing(x, weight, bias, residual, dtype):
+    """No rows, or rows of nothing: the sum is empty and no kernel runs."""
+    if x.shape[1] == 0 or weight.shape[0] == 0:
+        if x.shape[0] and weight.shape[0]:
+            raise ValueError("masked_linear_act: rows of at least one value")
+    y = x.new_empty((x.shape[0], weight.shape[0]), dtype=dtype)
+    # keeps every input in the graph, so that each gets a gradient of zeros
+    y = y + (x.sum() + weight.sum()
+             + (bias.sum() if bias is not None else 0)).to(dtype) * 0
+    return y if residual is None else (y + residual).to(residual.dtype)
 
 
 def synflow_linearize_(t: torch.Tensor):

@@ -178,6 +178,15 @@ class LinearMask(_MaskedMixin, nn.Linear):
         return TF.masked_linear(x, self.weight, self.mask, self.bias,
                                 self._fresh_cache(), self.compute_dtype)
 
+    def fused(self, x: torch.Tensor, residual=None, act=None, keep=None,
+              kept=None) -> torch.Tensor:
+        """``act(forward(x)) + residual`` in one product with an epilogue
+        (``functional.masked_linear_act``); ``keep="e4m3"`` holds what the
+        backward pass needs in 8 bits."""
+        return TF.masked_linear_act(
+            x, self.weight, self.mask, self.bias, residual, act,
+            self._fresh_cache(), self.compute_dtype, keep, kept)
+
 
 class Conv1dMask(_MaskedMixin, nn.Conv1d):
     """Linear-as-1x1-conv with weight mask (reference:
@@ -197,6 +206,15 @@ class Conv1dMask(_MaskedMixin, nn.Conv1d):
             x, self.weight.squeeze(-1), self.mask.squeeze(-1), self.bias,
             cache.squeeze(-1) if cache is not None else None,
             self.compute_dtype)
+
+    def fused(self, x: torch.Tensor, residual=None, act=None, keep=None,
+              kept=None) -> torch.Tensor:
+        """``LinearMask.fused``."""
+        cache = self._fresh_cache()
+        return TF.masked_linear_act(
+            x, self.weight.squeeze(-1), self.mask.squeeze(-1), self.bias,
+            residual, act, cache.squeeze(-1) if cache is not None else None,
+            self.compute_dtype, keep, kept)
 
 
 MASKED_LAYER_TYPES = (ConvMask, LinearMask, Conv1dMask)
