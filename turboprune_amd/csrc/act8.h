@@ -136,25 +136,14 @@ TP_DEVICE float rounded<float>(float v) { return v; }
 
 // ---- scale and codes -----------------------------------------------------
 // largest over the 4 lanes that hold one block (lanes 4k .. 4k+3)
-TP_DEVICE float quad_max(float v) {
-  int o = __builtin_amdgcn_mov_dpp(__float_as_int(v), 0xB1, 0xf, 0xf, true);
-  v = fmaxf(v, __int_as_float(o));   // quad_perm [1,0,3,2]
-  o = __builtin_amdgcn_mov_dpp(__float_as_int(v), 0x4E, 0xf, 0xf, true);
-  return fmaxf(v, __int_as_float(o));   // quad_perm [2,3,0,1]
-}
-
-TP_DEVICE float finite_abs(float v) {
-  float a = fabsf(v);
-  return a <= 3.402823466e38f ? a : 0.f;   // false for NaN and infinity
-}
-
-// largest finite magnitude of 8 values
-TP_DEVICE float amax8(const float (&v)[8]) {
-  float m = finite_abs(v[0]);
-#pragma unroll
-  for (int i = 1; i < 8; ++i) m = fmaxf(m, finite_abs(v[i]));
-  return m;
-}
+struct QuadMax {
+  TP_DEVICE float operator()(float v) const {
+    int o = __builtin_amdgcn_mov_dpp(__float_as_int(v), 0xB1, 0xf, 0xf, true);
+    v = fmaxf(v, __int_as_float(o));   // quad_perm [1,0,3,2]
+    o = __builtin_amdgcn_mov_dpp(__float_as_int(v), 0x4E, 0xf, 0xf, true);
+    return fmaxf(v, __int_as_float(o));   // quad_perm [2,3,0,1]
+  }
+};
 
 // e of the block: amax = m 2^k gives k - 8, one more where m > 1.75
 // (adding 0x1fffff carries into the exponent exactly then)
@@ -164,34 +153,54 @@ TP_DEVICE int block_exp(float amax) {
 }
 TP_DEVICE float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
-// 8 codes of values that 2^-e brings to 448 or less. An infinity becomes NaN
-// before the conversion, whose own answer for it is not relied on. At e = 120
-// the codes end at 240, since 256 * 2^120 is no finite float.
-TP_DEVICE uint2 encode8(const float (&v)[8], int e) {
-  float inv = pow2(-e), top = e < 120 ? 448.f : 240.f;
-  float s[8];
+typedef __attribute__((ext_vector_type(2))) short s16x2v;
+
+TP_DEVICE uint2 convert8(const float (&v)[8], float scale) {
+  s16x2v lo = {0, 0}, hi = {0, 0};
+  lo = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(lo, v[0], v[1], scale, false);
+  lo = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(lo, v[2], v[3], scale, true);
+  hi = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(hi, v[4], v[5], scale, false);
+  hi = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(hi, v[6], v[7], scale, true);
+  return make_uint2(__builtin_bit_cast(uint32_t, lo),
+                    __builtin_bit_cast(uint32_t, hi));
+}
+
+// The codes of a lane's 8 values and its block's e; `over` takes a lane's
+// number to the largest over the lanes of the block. The instructions do the
+// whole of it (1.5 to a value) but for blocks with infinities, with nothing
+// but NaN, or with magnitudes that 256 * 2^120, no finite float, would stand
+// for: those take the second path, all lanes of a block together.
+template <typename Over>
+TP_DEVICE uint2 encode8(const float (&v)[8], int& e, Over over) {
+  float m = fabsf(v[0]);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    float a = v[i] * inv;
-    s[i] = fabsf(a) <= 448.f ? __builtin_amdgcn_fmed3f(a, -top, top)
-                             : __uint_as_float(0x7fc00000u);
+  for (int i = 1; i < 8; ++i) m = fmaxf(m, fabsf(v[i]));   // passes NaN over
+  m = over(m);
+  if (m <= 3.1e38f) {
+    e = block_exp(m);
+    return convert8(v, pow2(e));
   }
-  int lo = __builtin_amdgcn_cvt_pk_fp8_f32(s[0], s[1], 0, false);
-  lo = __builtin_amdgcn_cvt_pk_fp8_f32(s[2], s[3], lo, true);
-  int hi = __builtin_amdgcn_cvt_pk_fp8_f32(s[4], s[5], 0, false);
-  hi = __builtin_amdgcn_cvt_pk_fp8_f32(s[6], s[7], hi, true);
-  return make_uint2((uint32_t)lo, (uint32_t)hi);
+  m = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    m = fmaxf(m, fabsf(v[i]) <= 3.402823466e38f ? fabsf(v[i]) : 0.f);
+  e = block_exp(over(m));
+  float top = e < 120 ? 3.402823466e38f : 240.f * pow2(120), s[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    s[i] = fabsf(v[i]) <= 3.402823466e38f
+               ? __builtin_amdgcn_fmed3f(v[i], -top, top)
+               : __uint_as_float(0x7fc00000u);
+  return convert8(s, pow2(e));
 }
 
 TP_DEVICE void decode8(uint2 c, float scale, float (&v)[8]) {
-  f32x2v a = __builtin_amdgcn_cvt_pk_f32_fp8((int)c.x, false);
-  f32x2v b = __builtin_amdgcn_cvt_pk_f32_fp8((int)c.x, true);
-  f32x2v d = __builtin_amdgcn_cvt_pk_f32_fp8((int)c.y, false);
-  f32x2v e = __builtin_amdgcn_cvt_pk_f32_fp8((int)c.y, true);
-  v[0] = a[0] * scale; v[1] = a[1] * scale;
-  v[2] = b[0] * scale; v[3] = b[1] * scale;
-  v[4] = d[0] * scale; v[5] = d[1] * scale;
-  v[6] = e[0] * scale; v[7] = e[1] * scale;
+  f32x2v a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(c.x, scale, false);
+  f32x2v b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(c.x, scale, true);
+  f32x2v d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(c.y, scale, false);
+  f32x2v e = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(c.y, scale, true);
+  v[0] = a[0]; v[1] = a[1]; v[2] = b[0]; v[3] = b[1];
+  v[4] = d[0]; v[5] = d[1]; v[6] = e[0]; v[7] = e[1];
 }
 
 // a code's value within T's finite range: in fp16 the largest magnitudes
@@ -255,6 +264,25 @@ TP_DEVICE float bell_exp(float z) {   // exp(-z^2/2) = 2^(-z^2 / (2 ln 2))
 TP_DEVICE float gelu(float z) {
   float q = normal_tail(fabsf(z), bell_exp(z));
   return z * (z < 0.f ? q : 1.f - q);
+}
+// The same for 16-bit results behind a product, where these instructions
+// bound the epilogue: gelu(z) = max(z, 0) - t Phi(-t), t = |z|, with
+// Phi(-t) = 2^-h(t), h a polynomial (fitted here over [0, 6.5] and exactly 1
+// at 0): 15 instruction slots a value against 25. Off by 5e-6 of t Phi(-t) up
+// to t = 4, by 5e-5 up to 6.5; behind it t stays at 6.5 and the result within
+// 3e-10 of max(z, 0).
+TP_DEVICE float gelu_short(float z) {
+  float t = fminf(fabsf(z), 6.5f);
+  float h = 1.7347767879982712e-06f;
+  h = fmaf(h, t, -5.966168100712821e-05f);
+  h = fmaf(h, t, 0.00091591477394104f);
+  h = fmaf(h, t, -0.008453256450593472f);
+  h = fmaf(h, t, 0.05385367572307587f);
+  h = fmaf(h, t, 0.4585675299167633f);
+  h = fmaf(h, t, 1.1512086391448975f);
+  float q = __builtin_amdgcn_exp2f(-fmaf(h, t, 1.f));
+  // z + |z| is 2 max(z, 0), and NaN where z is
+  return fmaf(-t, q, 0.5f * (z + fabsf(z)));
 }
 TP_DEVICE float gelu_slope(float z) {
   float e = bell_exp(z);

@@ -60,10 +60,10 @@ __global__ __launch_bounds__(kBlock) void keep_kernel(
   }
 #pragma unroll
   for (int u = 0; u < kPer; ++u) {
-    int e = block_exp(quad_max(amax8(v[u])));
-    int n = a[u].n;
+    int e, n = a[u].n;
+    uint2 c = encode8(v[u], e, QuadMax());
     if (n <= 0) continue;
-    store_codes(codes + a[u].off, n, encode8(v[u], e));
+    store_codes(codes + a[u].off, n, c);
     if ((threadIdx.x & 3) == 0) scales[a[u].blk] = (uint8_t)(e + 127);
     if constexpr (OP == kGelu) {
       float o[8];

@@ -12,6 +12,8 @@
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPException.h>
 
+#include <type_traits>
+
 #include "act8.h"
 
 namespace turboprune {
@@ -51,7 +53,7 @@ struct Epi {
   void* z;               // (M,N) kept pre-activation: 16-bit values or codes
   uint8_t* zscale;       // its scales; null: z holds 16-bit values
   const float* mask;     // weight gradient: 0/1 per value, or null
-  int bias_f32, res_f32, out_f32, act;
+  int bias_f32, res_f32, out_f32;
 };
 
 // C[q][p] = sum_k Q P. An operand is a matrix of 16-bit values, with
@@ -71,19 +73,28 @@ struct Mm {
   Epi e;
 };
 
-constexpr int kBK = 64;
-
-// LDS image of a RowK tile: rows of 64 values (128 B); the 16-byte chunk c of
-// row r sits at c ^ (r & 7), so the 16 rows of a fragment read spread over
-// all banks. Of a ColK tile: 64 rows (along k) of W values; the 32-byte block
-// b of row r sits at b ^ f(r) with f(r) = (r & 3) | (r >> 3 & 1) << 2: the
-// rows that one transposing read touches together then differ in bank.
-template <int W, bool TR>
+// LDS image of a kRowK tile: rows of BK values (64 or 128 B); the 16-byte
+// chunk c of row r sits at c ^ (r / (256 B / row)), so that the 16 rows of a
+// fragment read spread over all 64 banks. Of a kColK tile: BK rows (along k)
+// of W values; the 32-byte block b of row r sits at b ^ f(r) with
+// f(r) = (r & 3) | (r >> 3 & 1) << 2: the rows that one transposing read
+// touches together then differ in bank.
+template <int W, int BK, bool TR>
 struct Tile {
-  static constexpr int kBytes = W * kBK * 2;
-  static constexpr int kRow = TR ? W * 2 : kBK * 2;
+  static constexpr int kBytes = W * BK * 2;
   static constexpr int kLoads = kBytes / 1024;   // wave-wide 16 B loads
+  static constexpr int kChunks = BK / 8;         // of a kRowK row
+  TP_DEVICE static int swap(int row) {
+    return BK == 64 ? row / 2 % 8 : (row / 8 % 2) * 3;
+  }
 };
+
+// f(r) of a kColK tile; rows of 64 values, two to 256 B, need only two bits
+template <int W>
+TP_DEVICE int col_swap(int row) {
+  return W == 64 ? (row >> 1 & 1) | (row >> 3 & 1) << 1
+                 : (row & 3) | (row >> 3 & 1) << 2;
+}
 
 typedef __amdgpu_buffer_rsrc_t rsrc_t;
 TP_DEVICE rsrc_t rsrc(const void* p, int64_t bytes) {
@@ -95,37 +106,37 @@ constexpr int kOut = 0x7ffffff8;   // an offset that no buffer reaches
 
 // Wave `w` of NW brings its share of a tile into LDS with asynchronous
 // 16-byte loads; what lies outside the matrix arrives as zeros.
-template <int W, bool TR, int NW>
+template <int W, int BK, bool TR, int NW>
 TP_DEVICE void stage(TP_LDS char* dst, const char* base, int64_t ld,
                      int first, int count, int kt, int K, int wave,
                      int lane) {
-  constexpr int PER = Tile<W, TR>::kLoads / NW;
-  static_assert(PER * NW == Tile<W, TR>::kLoads, "loads divide evenly");
+  typedef Tile<W, BK, TR> L;
+  constexpr int PER = L::kLoads / NW;
+  static_assert(PER * NW == L::kLoads, "loads divide evenly");
   if constexpr (!TR) {
     int rows = min(W, count - first);
     rsrc_t r = rsrc(base + (int64_t)first * ld,
                     (int64_t)(rows - 1) * ld + (K + 7) / 8 * 16);
-    int c = (lane & 7) ^ (lane >> 3);
-    int off = (lane >> 3) * (int)ld + c * 16;
-    if (kt * kBK + c * 8 >= K) off = kOut;
+    constexpr int RPL = 64 / L::kChunks;   // rows of one load
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      int row8 = wave * PER + i;
+      int row = (wave * PER + i) * RPL + lane / L::kChunks;
+      int c = lane % L::kChunks ^ L::swap(row);
+      int off = row * (int)ld + c * 16;
       __builtin_amdgcn_raw_ptr_buffer_load_lds(
-          r, (TP_LDS void*)(dst + row8 * 1024), 16,
-          off == kOut ? kOut : off + row8 * 8 * (int)ld, kt * kBK * 2, 0, 0);
+          r, (TP_LDS void*)(dst + (wave * PER + i) * 1024), 16,
+          kt * BK + c * 8 < K ? off : kOut, kt * BK * 2, 0, 0);
     }
   } else {
-    int k0 = kt * kBK, rows = min(kBK, K - k0);
-    constexpr int RB = W * 2;             // bytes of a row of the tile
-    constexpr int LPR = RB / 16;          // lanes to a row
+    int k0 = kt * BK, rows = min(BK, K - k0);
+    constexpr int LPR = W * 2 / 16;       // lanes to a row
     rsrc_t r = rsrc(base + (int64_t)k0 * ld + (int64_t)first * 2,
                     (int64_t)(rows - 1) * ld + (int64_t)(count - first) * 2);
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       int chunk = (wave * PER + i) * 64 + lane;
       int row = chunk / LPR, c = chunk % LPR;
-      int f = (row & 3) | ((row >> 3 & 1) << 2);
+      int f = col_swap<W>(row);
       int col = ((c >> 1) ^ f) * 32 + (c & 1) * 16;
       __builtin_amdgcn_raw_ptr_buffer_load_lds(
           r, (TP_LDS void*)(dst + (wave * PER + i) * 1024), 16,
@@ -136,16 +147,16 @@ TP_DEVICE void stage(TP_LDS char* dst, const char* base, int64_t ld,
 
 // Fragment of 16 rows (columns) from `at` and 32 values of k from ks * 32:
 // lane l holds number l % 16, k from (l / 16) * 8.
-template <int W, bool TR>
+template <int W, int BK, bool TR>
 TP_DEVICE s16x8 frag(TP_LDS const char* t, int at, int ks, int lane) {
   int g = lane >> 4, i = lane & 15;
   if constexpr (!TR) {
     int row = at + i;
-    int c = (ks * 4 + g) ^ (row & 7);
-    return *reinterpret_cast<TP_LDS const s16x8*>(t + row * 128 + c * 16);
+    int c = (ks * 4 + g) ^ Tile<W, BK, TR>::swap(row);
+    return *reinterpret_cast<TP_LDS const s16x8*>(t + row * (BK * 2) + c * 16);
   } else {
-    int row = ks * 32 + g * 8 + (i >> 2);
-    int f = (i >> 2) | ((g & 1) << 2);
+    int row = ks * 32 + g * 8 + (i >> 2);   // and 4 rows on: the same swap
+    int f = col_swap<W>(row);
     TP_LDS const char* a =
         t + row * (W * 2) + (((at >> 4) ^ f) * 32) + (i & 3) * 8;
     s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((TP_LDS s16x4*)a);
@@ -158,9 +169,10 @@ TP_DEVICE s16x8 frag(TP_LDS const char* t, int at, int ks, int lane) {
 // kCodes tiles go through registers: 16 codes of one row, with their scale,
 // become 16 values in two LDS stores. A code times a power of two is exact in
 // bf16; in fp16 it is brought into range first.
-template <typename T, int W, int THREADS>
+template <typename T, int W, int BK, int THREADS>
 struct CodeTile {
-  static constexpr int kPer = W * kBK / 16 / THREADS;
+  static constexpr int kAll = W * BK / 16;
+  static constexpr int kPer = (kAll + THREADS - 1) / THREADS;
   u32x4 code[kPer];
   uint32_t scale[kPer];
 
@@ -169,8 +181,8 @@ struct CodeTile {
     for (int i = 0; i < kPer; ++i) {
       int at = i * THREADS + threadIdx.x;
       int row = at / (W / 16), col = first + at % (W / 16) * 16;
-      int64_t k = (int64_t)kt * kBK + row;
-      int n = k < a.K ? a.np - col : 0;
+      int64_t k = (int64_t)kt * BK + row;
+      int n = k < a.K && at < kAll ? a.np - col : 0;
       const uint8_t* p = (const uint8_t*)a.p + k * a.ldp + col;
       uint2 lo = load_codes(p, n), hi = load_codes(p + 8, n - 8);
       code[i] = u32x4{lo.x, lo.y, hi.x, hi.y};
@@ -182,8 +194,9 @@ struct CodeTile {
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
       int at = i * THREADS + threadIdx.x;
+      if (kAll % THREADS && at >= kAll) break;
       int row = at / (W / 16), blk = at % (W / 16);
-      int f = (row & 3) | ((row >> 3 & 1) << 2);
+      int f = col_swap<W>(row);
       float sc = __uint_as_float(scale[i] << 23);
       u32x4 v[2];
 #pragma unroll
@@ -219,67 +232,82 @@ TP_DEVICE void wait_and_meet() {
                : "memory");
 }
 
-TP_DEVICE float lanes_max_16_32(float v) {
-  v = fmaxf(v, __shfl_xor(v, 16, kWave));
-  return fmaxf(v, __shfl_xor(v, 32, kWave));
+struct LanesMax {   // over lanes l, l^16, l^32, l^48
+  TP_DEVICE float operator()(float v) const {
+    uint32_t u = __float_as_uint(v);
+    auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    u = __float_as_uint(v);
+    a = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    return fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  }
+};
+
+// What follows the sum: nothing but the residual, GELU with z kept in 16 bits
+// (or not at all), GELU with z kept in 8.
+enum { kNoAct = 0, kGelu = 1, kGelu8 = 2 };
+
+template <bool FULL, typename T>
+TP_DEVICE void put8(T* p, int n, const float (&v)[8]) {
+  if constexpr (FULL)
+    store8(p, v);
+  else
+    store8n(p, n, v);
+}
+template <bool FULL, typename T>
+TP_DEVICE void add8(const T* p, int n, float (&v)[8]) {
+  float r[8];
+  if constexpr (FULL)
+    load8(p, r);
+  else
+    load8n(p, n, r);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] += r[i];
 }
 
-template <typename T>
-TP_DEVICE void epilogue8(const Epi& e, int64_t row, int col, int n, int N,
-                         float (&v)[8]) {
-  // v: 8 neighbouring columns of one row; n of them exist (<= 0: none). The
-  // lanes l, l^16, l^32 and l^48 hold one 32-column block.
-  if (e.bias) {
-    float b[8];
-    if (e.bias_f32)
-      load8n((const float*)e.bias + col, n, b);
-    else
-      load8n((const T*)e.bias + col, n, b);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] += b[i];
-  }
-  if (e.z) {
-    if (e.zscale) {
-      int x = block_exp(lanes_max_16_32(amax8(v)));
-      if (n > 0) {
-        store_codes((uint8_t*)e.z + row * N + col, n, encode8(v, x));
-        if ((col & 31) == 0)
-          e.zscale[row * ((N + 31) / 32) + col / 32] = (uint8_t)(x + 127);
-      }
-    } else {
-      store8n((T*)e.z + row * N + col, n, v);
+// v: the sums of 8 neighbouring columns of one row; n of them exist (<= 0:
+// none; FULL: all). The lanes l, l^16, l^32 and l^48 hold one 32-column block.
+template <typename T, int ACT, bool FULL>
+TP_DEVICE void epilogue8(const Epi& e, int64_t at, int64_t blk, int n,
+                         bool first, float (&v)[8]) {
+  if constexpr (ACT == kGelu8) {
+    int x;
+    uint2 q = encode8(v, x, LanesMax());
+    if (FULL || n > 0) {
+      store_codes((uint8_t*)e.z + at, FULL ? 8 : n, q);
+      if (first) e.zscale[blk] = (uint8_t)(x + 127);
     }
   }
-  if (e.act)
+  if constexpr (ACT == kGelu)
+    if (e.z) put8<FULL>((T*)e.z + at, n, v);
+  if constexpr (ACT != kNoAct)
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = gelu(v[i]);
+    for (int i = 0; i < 8; ++i) v[i] = gelu_short(v[i]);
   if (e.res) {
-    float r[8];
     if (e.res_f32)
-      load8n((const float*)e.res + row * N + col, n, r);
+      add8<FULL>((const float*)e.res + at, n, v);
     else
-      load8n((const T*)e.res + row * N + col, n, r);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] += r[i];
+      add8<FULL>((const T*)e.res + at, n, v);
   }
-  if (e.mask) {
-    float m[8];
-    load8n(e.mask + row * N + col, n, m);
+  if constexpr (ACT == kNoAct)
+    if (e.mask) {
+      float m[8];
+      load8n(e.mask + at, n, m);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = m[i] != 0.f ? v[i] : 0.f;
-  }
+      for (int i = 0; i < 8; ++i) v[i] = m[i] != 0.f ? v[i] : 0.f;
+    }
   if (e.out_f32)
-    store8n((float*)e.out + row * N + col, n, v);
+    put8<FULL>((float*)e.out + at, n, v);
   else
-    store8n((T*)e.out + row * N + col, n, v);
+    put8<FULL>((T*)e.out + at, n, v);
 }
 
-template <typename T, int BQ, int BP, int WQ, int WP, int QF, int PF,
-          int STAGES>
-__global__ __launch_bounds__(WQ * WP * 64) void mm_kernel(Mm a) {
+template <typename T, int BQ, int BP, int BK, int WQ, int WP, int QF, int PF,
+          int STAGES, int MINW, int ACT>
+__global__ __launch_bounds__(WQ * WP * 64, MINW) void mm_kernel(Mm a) {
   constexpr int NW = WQ * WP;
   constexpr bool QTR = QF != kRowK, PTR = PF != kRowK;
-  constexpr int QB = Tile<BQ, QTR>::kBytes, PB = Tile<BP, PTR>::kBytes;
+  constexpr int QB = Tile<BQ, BK, QTR>::kBytes, PB = Tile<BP, BK, PTR>::kBytes;
   // asynchronous loads of a wave for one k-tile
   constexpr int LOADS = (QB + (PF == kCodes ? 0 : PB)) / 1024 / NW;
   constexpr int MI = BQ / WQ / 16, NI = BP / WP / 16;
@@ -300,20 +328,34 @@ __global__ __launch_bounds__(WQ * WP * 64) void mm_kernel(Mm a) {
   int wq = wave / WP * (BQ / WQ), wp = wave % WP * (BP / WP);
 
   int kt0 = blockIdx.y * a.kper;
-  int kt1 = min((a.K + kBK - 1) / kBK, kt0 + a.kper);
+  int kt1 = min((a.K + BK - 1) / BK, kt0 + a.kper);
 
   auto place = [&](int kt) {
     return lds + (kt - kt0) % STAGES * (QB + PB);
   };
   auto fetch = [&](int kt) {
     TP_LDS char* b = place(kt);
-    stage<BQ, QTR, NW>(b, a.q, a.ldq, m0, a.nq, kt, a.K, wave, lane);
+    stage<BQ, BK, QTR, NW>(b, a.q, a.ldq, m0, a.nq, kt, a.K, wave, lane);
     if constexpr (PF != kCodes)
-      stage<BP, PTR, NW>(b + QB, a.p, a.ldp, n0, a.np, kt, a.K, wave, lane);
+      stage<BP, BK, PTR, NW>(b + QB, a.p, a.ldp, n0, a.np, kt, a.K, wave, lane);
   };
-  CodeTile<T, BP, NW * 64> ct;
+  CodeTile<T, BP, BK, NW * 64> ct;
 
-  f32x4 acc[NI][MI] = {};
+  // the sum begins with the bias: lane l holds four columns from l / 16 * 4
+  f32x4 acc[NI][MI];
+#pragma unroll
+  for (int i = 0; i < NI; ++i) {
+    f32x4 b = {};
+    int col = n0 + wp + i * 16 + (lane >> 4) * 4;
+    if (a.e.bias)
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (col + k < a.N)
+          b[k] = a.e.bias_f32 ? ((const float*)a.e.bias)[col + k]
+                              : to_float<T>(((const T*)a.e.bias)[col + k]);
+#pragma unroll
+    for (int j = 0; j < MI; ++j) acc[i][j] = b;
+  }
 #pragma unroll
   for (int s = 0; s < STAGES - 1; ++s)
     if (kt0 + s < kt1) fetch(kt0 + s);
@@ -339,14 +381,14 @@ __global__ __launch_bounds__(WQ * WP * 64) void mm_kernel(Mm a) {
     }
     TP_LDS const char* b = place(kt);
 #pragma unroll
-    for (int ks = 0; ks < kBK / 32; ++ks) {
+    for (int ks = 0; ks < BK / 32; ++ks) {
       s16x8 fq[MI], fp[NI];
 #pragma unroll
       for (int i = 0; i < MI; ++i)
-        fq[i] = frag<BQ, QTR>(b, wq + i * 16, ks, lane);
+        fq[i] = frag<BQ, BK, QTR>(b, wq + i * 16, ks, lane);
 #pragma unroll
       for (int i = 0; i < NI; ++i)
-        fp[i] = frag<BP, PTR>(b + QB, wp + i * 16, ks, lane);
+        fp[i] = frag<BP, BK, PTR>(b + QB, wp + i * 16, ks, lane);
 #pragma unroll
       for (int i = 0; i < NI; ++i)
 #pragma unroll
@@ -359,25 +401,35 @@ __global__ __launch_bounds__(WQ * WP * 64) void mm_kernel(Mm a) {
   // (l / 16) * 4. Swapping 16-lane groups between two neighbouring fragments
   // leaves every lane with eight neighbouring columns: one 16-byte store.
   a.e.out = (char*)a.e.out + (int64_t)blockIdx.y * a.M * a.N * 4;
-  int g = lane >> 4;
+  int g = lane >> 4, nblk = (a.N + 31) / 32;
+  auto finish = [&](auto full) {
+    constexpr bool FULL = decltype(full)::value;
 #pragma unroll
-  for (int j = 0; j < MI; ++j) {
-    int row = m0 + wq + j * 16 + (lane & 15);
+    for (int j = 0; j < MI; ++j) {
+      int row = m0 + wq + j * 16 + (lane & 15);
+      int c0 = n0 + wp + (g & 1) * 16 + (g >> 1) * 8;
+      int64_t at = (int64_t)row * a.N + c0;
+      int64_t blk = (int64_t)row * nblk + (n0 + wp) / 32;
 #pragma unroll
-    for (int i = 0; i < NI; i += 2) {
-      float v[8];
+      for (int i = 0; i < NI; i += 2) {
+        float v[8];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        auto s = __builtin_amdgcn_permlane16_swap(
-            __float_as_uint(acc[i][j][k]), __float_as_uint(acc[i + 1][j][k]),
-            false, false);
-        v[k] = __uint_as_float(s[0]);
-        v[4 + k] = __uint_as_float(s[1]);
+        for (int k = 0; k < 4; ++k) {
+          auto s = __builtin_amdgcn_permlane16_swap(
+              __float_as_uint(acc[i][j][k]),
+              __float_as_uint(acc[i + 1][j][k]), false, false);
+          v[k] = __uint_as_float(s[0]);
+          v[4 + k] = __uint_as_float(s[1]);
+        }
+        epilogue8<T, ACT, FULL>(a.e, at + i * 16, blk + i / 2,
+                                row < a.M ? a.N - c0 - i * 16 : 0, g == 0, v);
       }
-      int col = n0 + wp + i * 16 + (g & 1) * 16 + (g >> 1) * 8;
-      epilogue8<T>(a.e, row, col, row < a.M ? a.N - col : 0, a.N, v);
     }
-  }
+  };
+  if (m0 + BQ <= a.M && n0 + BP <= a.N && a.N % 8 == 0)
+    finish(std::true_type());
+  else
+    finish(std::false_type());
 }
 
 // sum of the slabs of a split product, masked and rounded
@@ -467,8 +519,17 @@ __global__ __launch_bounds__(1024) void colsum_kernel(
   __shared__ float sum[16][64];
   int c = blockIdx.x * 64 + (threadIdx.x & 63), k = threadIdx.x >> 6;
   float v = 0.f;
-  if (c < C)
-    for (int r = k; r < n; r += 16) v += part[(int64_t)r * C + c];
+  if (c < C) {
+    int r = k;
+    for (; r + 7 * 16 < n; r += 8 * 16) {
+      float t[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) t[i] = part[(int64_t)(r + i * 16) * C + c];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v += t[i];
+    }
+    for (; r < n; r += 16) v += part[(int64_t)r * C + c];
+  }
   sum[k][threadIdx.x & 63] = v;
   __syncthreads();
   if (k == 0 && c < C) {
@@ -491,6 +552,35 @@ __global__ __launch_bounds__(kBlock) void pad_kernel(
   float v[8];
   load8n(x + row * ldx + c, C - c, v);
   store8(out + (row * cpr) * 8 + c, v);
+}
+
+// w (N, K), rows ldw apart, to (K, N8) with zeros behind N: 64 x 64 tiles
+// through LDS
+template <typename T>
+__global__ __launch_bounds__(kBlock) void turn_kernel(
+    const T* __restrict__ w, T* __restrict__ out, int64_t ldw, int N, int K,
+    int N8) {
+  __shared__ T tile[64][66];
+  int n0 = blockIdx.x * 64, k0 = blockIdx.y * 64;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    int at = i * kBlock + threadIdx.x, r = at / 8, c = at % 8 * 8;
+    int n = n0 + r;
+    float v[8];
+    load8n(w + (int64_t)n * ldw + k0 + c, n < N ? K - k0 - c : 0, v);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) tile[c + j][r] = from_float<T>(v[j]);
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    int at = i * kBlock + threadIdx.x, r = at / 8, c = at % 8 * 8;
+    if (k0 + r >= K || n0 + c >= N8) continue;
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = to_float<T>(tile[r][c + j]);
+    store8(out + (int64_t)(k0 + r) * N8 + n0 + c, v);
+  }
 }
 
 bool is16(at::ScalarType t) { return t == at::kBFloat16 || t == at::kHalf; }
@@ -535,20 +625,70 @@ int64_t row_bytes(const at::Tensor& t) {
   return (t.size(0) <= 1 ? t.size(1) : t.stride(0)) * 2;
 }
 
-template <typename T, int BQ, int BP, int WQ, int WP, int QF, int PF, int ST>
-void launch_mm(Mm a, int slabs) {
+template <typename T, int BQ, int BP, int BK, int WQ, int WP, int QF, int PF,
+          int ST, int MINW, int ACT = kNoAct>
+void launch_mm(Mm a, int slabs = 1) {
   a.tiles_n = (a.N + BP - 1) / BP;
   a.tiles = (a.M + BQ - 1) / BQ * a.tiles_n;
-  int kt = (a.K + kBK - 1) / kBK;
+  int kt = (a.K + BK - 1) / BK;
   a.kper = (kt + slabs - 1) / slabs;
-  mm_kernel<T, BQ, BP, WQ, WP, QF, PF, ST>
+  mm_kernel<T, BQ, BP, BK, WQ, WP, QF, PF, ST, MINW, ACT>
       <<<dim3(a.tiles, slabs), WQ * WP * 64, 0, current()>>>(a);
   C10_HIP_KERNEL_LAUNCH_CHECK();
 }
 
-template <typename T, int QF, int PF>
-void run_mm(const Mm& a, int slabs) {
-  launch_mm<T, 128, 128, 2, 2, QF, PF, 2>(a, slabs);
+int64_t tiles_of(const Mm& a, int q, int p) {
+  return (int64_t)((a.M + q - 1) / q) * ((a.N + p - 1) / p);
+}
+
+// Both operands along the sum. 256 x 256 by 16 waves moves the fewest bytes
+// into LDS per product but needs about a CU each to pay: 50432x1536x384 in 92
+// us against 111 with 128 x 128, but 12608x1536x384 (300 tiles, two rounds for
+// little more than one) 32 against 26. Short products end soonest in many
+// small tiles: 1576x768x768 10.2 us in 64 x 64, 12.0 in 128 x 128;
+// 3152x1536x384 (1200 small tiles) 13.8 against 12.9.
+template <typename T, int ACT>
+void run_rows(const Mm& a) {
+  if (tiles_of(a, 64, 64) <= 600)
+    return launch_mm<T, 64, 64, 64, 2, 2, kRowK, kRowK, 2, 1, ACT>(a);
+  int64_t t = tiles_of(a, 256, 256);
+  if (t >= 200 && (a.K >= 512 || t >= 768))
+    return launch_mm<T, 256, 256, 64, 4, 4, kRowK, kRowK, 2, 4, ACT>(a);
+  launch_mm<T, 128, 128, 64, 2, 4, kRowK, kRowK, 2, 2, ACT>(a);
+}
+
+// Both across the sum (weight gradients), in slabs of it: as many as fill the
+// chip, none shorter than four k-tiles. 4096x1024 over 25216 rows takes 204 us
+// in 256 x 256 tiles and 235 in 128 x 128; 1536x384 over 50432 rows 87 us in
+// 128 x 128 and 97 in 256 x 256, whose third column tile is half empty.
+// Codes go through registers, which 16 waves leave too few of: 8 waves there
+// (253 us against 285; 128 x 128 336).
+struct Split {
+  int tile, slabs;
+};
+Split split_of(const Mm& a) {
+  int big = (int)std::min<int64_t>(tiles_of(a, 256, 256), 1 << 20);
+  int64_t kt = (a.K + 63) / 64;
+  bool even = (a.M % 256 == 0 || a.M % 256 > 192 || a.M > 2048) &&
+              (a.N % 256 == 0 || a.N % 256 > 192 || a.N > 2048);
+  int tile = big >= 12 && even ? 256 : 128;
+  if (tile == 128 && tiles_of(a, 128, 128) * (kt / 4) < 128) tile = 64;
+  int64_t tiles = tiles_of(a, tile, tile);
+  int64_t fill = tile == 256 ? 256 : 512;
+  int64_t most = std::max<int64_t>(1, kt / (tile == 64 ? 2 : 4));
+  return {tile, (int)std::max<int64_t>(1, std::min(most, fill / tiles))};
+}
+template <typename T, int PF>
+void run_cols(const Mm& a, Split s) {
+  if (s.tile == 256) {
+    if constexpr (PF == kCodes)
+      return launch_mm<T, 256, 256, 64, 2, 4, kColK, PF, 2, 2>(a, s.slabs);
+    else
+      return launch_mm<T, 256, 256, 64, 4, 4, kColK, PF, 2, 4>(a, s.slabs);
+  }
+  if (s.tile == 128)
+    return launch_mm<T, 128, 128, 64, 2, 2, kColK, PF, 2, 2>(a, s.slabs);
+  launch_mm<T, 64, 64, 64, 2, 2, kColK, PF, 2, 1>(a, s.slabs);
 }
 
 void check_size(int64_t M, int64_t N, int64_t K) {
@@ -610,7 +750,6 @@ linear_act_fwd(const at::Tensor& x, const at::Tensor& w,
   if (zs) a.e.zscale = (uint8_t*)zs->data_ptr();
   a.e.out = y.data_ptr();
   a.e.out_f32 = ot == at::kFloat;
-  a.e.act = act;
   a.q = (const char*)xl.data_ptr();
   a.p = (const char*)wl.data_ptr();
   a.ldq = row_bytes(xl);
@@ -618,7 +757,15 @@ linear_act_fwd(const at::Tensor& x, const at::Tensor& w,
   a.nq = a.M = (int)M;
   a.np = a.N = (int)N;
   a.K = (int)K;
-  by16(st, [&](auto t) { run_mm<decltype(t), kRowK, kRowK>(a, 1); });
+  by16(st, [&](auto t) {
+    using T = decltype(t);
+    if (!act)
+      run_rows<T, kNoAct>(a);
+    else if (zs)
+      run_rows<T, kGelu8>(a);
+    else
+      run_rows<T, kGelu>(a);
+  });
   return {y, z, zs};
 }
 
@@ -716,19 +863,42 @@ linear_act_bwd(const at::Tensor& dy_in, const c10::optional<at::Tensor>& z,
     }
   }
   if (want_dx) {
-    auto wl = loadable(w);
     dx = at::empty({M, K}, opt);
     Mm a{};
     a.q = (const char*)dz.data_ptr();
     a.ldq = ldz * 2;
     a.nq = a.M = (int)M;
-    a.p = (const char*)wl.data_ptr();
-    a.ldp = row_bytes(wl);
-    a.np = (int)wl.size(1);
     a.N = (int)K;
     a.K = (int)N;
     a.e.out = dx->data_ptr();
-    by16(st, [&](auto t) { run_mm<decltype(t), kRowK, kColK>(a, 1); });
+    // w along the sum: turned over first where the product is long enough to
+    // win it back (50432x384x1536: 95 us and 3 for the turn, 111 across;
+    // 25216x1024x4096: 214 and 5, 282 across)
+    if (tiles_of(a, 64, 64) > 600) {
+      auto ws = K <= 1 || w.stride(1) == 1 ? w : w.contiguous();
+      auto wt = at::empty({K, ldz}, opt);
+      by16(st, [&](auto t) {
+        using T = decltype(t);
+        turn_kernel<T><<<dim3((unsigned)((ldz + 63) / 64),
+                              (unsigned)((K + 63) / 64)),
+                         kBlock, 0, current()>>>(
+            (const T*)ws.data_ptr(), (T*)wt.data_ptr(), ws.stride(0), (int)N,
+            (int)K, (int)ldz);
+        C10_HIP_KERNEL_LAUNCH_CHECK();
+        a.p = (const char*)wt.data_ptr();
+        a.ldp = ldz * 2;
+        a.np = (int)K;
+        run_rows<T, kNoAct>(a);
+      });
+    } else {
+      auto wl = loadable(w);
+      a.p = (const char*)wl.data_ptr();
+      a.ldp = row_bytes(wl);
+      a.np = (int)wl.size(1);
+      by16(st, [&](auto t) {
+        launch_mm<decltype(t), 64, 64, 64, 2, 2, kRowK, kColK, 2, 1>(a);
+      });
+    }
   }
   if (dw_type.has_value()) {
     dw = at::empty({N, K}, opt.dtype(*dw_type));
@@ -772,10 +942,8 @@ linear_act_bwd(const at::Tensor& dy_in, const c10::optional<at::Tensor>& z,
                   "linear_act_bwd: float32 mask of w's shape");
       m = mask->contiguous();
     }
-    // Few output tiles, a long sum: slabs of it in fp32, joined afterwards.
-    int tiles = (int)((N + 127) / 128 * ((K + 127) / 128));
-    int kts = (int)((M + kBK - 1) / kBK);
-    int slabs = std::max(1, std::min(kts / 4, 512 / tiles));
+    Split split = split_of(a);
+    int slabs = split.slabs;
     bool join = slabs > 1 || *dw_type != st;
     at::Tensor part2;
     if (join) {
@@ -789,9 +957,9 @@ linear_act_bwd(const at::Tensor& dy_in, const c10::optional<at::Tensor>& z,
     by16(st, [&](auto t) {
       using T = decltype(t);
       if (xscale.has_value())
-        run_mm<T, kColK, kCodes>(a, slabs);
+        run_cols<T, kCodes>(a, split);
       else
-        run_mm<T, kColK, kColK>(a, slabs);
+        run_cols<T, kColK>(a, split);
     });
     if (join) {
       int64_t n = N * K;

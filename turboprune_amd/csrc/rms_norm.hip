@@ -105,9 +105,10 @@ __global__ __launch_bounds__(kBlock) void rms_fwd_kernel(NormFwd p) {
       for (int i = 0; i < 8; ++i) v[j][i] = v[j][i] * rstd * w[i];
       store8n(y + c, n, v[j]);
       if (p.codes) {
-        int e = block_exp(quad_max(amax8(v[j])));
+        int e;
+        uint2 q = encode8(v[j], e, QuadMax());
         if (n > 0) {
-          store_codes(p.codes + row * p.C + c, n, encode8(v[j], e));
+          store_codes(p.codes + row * p.C + c, n, q);
           if ((t & 3) == 0)
             p.scales[row * sblk + c / kBlk] = (uint8_t)(e + 127);
         }
@@ -214,8 +215,18 @@ __global__ __launch_bounds__(1024) void rms_dw_kernel(
   __shared__ float sum[16][64];
   int c = blockIdx.x * 64 + (threadIdx.x & 63), k = threadIdx.x >> 6;
   float v = 0.f;
-  if (c < C)
-    for (int r = k; r < n; r += 16) v += part[(int64_t)r * C + c];
+  if (c < C) {
+    // eight loads in flight; one at a time is all latency
+    int r = k;
+    for (; r + 7 * 16 < n; r += 8 * 16) {
+      float t[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) t[i] = part[(int64_t)(r + i * 16) * C + c];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v += t[i];
+    }
+    for (; r < n; r += 16) v += part[(int64_t)r * C + c];
+  }
   sum[k][threadIdx.x & 63] = v;
   __syncthreads();
   if (k == 0 && c < C) {
@@ -266,9 +277,10 @@ __global__ __launch_bounds__(kBlock) void rms_fwd_long_kernel(NormFwd p) {
       for (int i = 0; i < 8; ++i) v[i] = v[i] * rstd * w[i];
       store8n((TY*)p.y + row * p.C + c, n, v);
       if (p.codes) {
-        int e = block_exp(quad_max(amax8(v)));
+        int e;
+        uint2 q = encode8(v, e, QuadMax());
         if (n > 0) {
-          store_codes(p.codes + row * p.C + c, n, encode8(v, e));
+          store_codes(p.codes + row * p.C + c, n, q);
           if ((threadIdx.x & 3) == 0)
             p.scales[row * sblk + c / kBlk] = (uint8_t)(e + 127);
         }
