@@ -43,6 +43,7 @@ sources = [
     os.path.join(CSRC, "act8.hip"),
     os.path.join(CSRC, "rms_norm.hip"),
     os.path.join(CSRC, "linear_act.hip"),
+    os.path.join(CSRC, "autograd_ops.cpp"),
 ]
 
 # the device objects carry no header dependencies of their own: a macro that

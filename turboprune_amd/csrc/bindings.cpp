@@ -98,6 +98,19 @@ rms_fwd(const at::Tensor&, const c10::optional<at::Tensor>&,
 std::tuple<at::Tensor, c10::optional<at::Tensor>, at::Tensor> rms_bwd(
     const at::Tensor&, const c10::optional<at::Tensor>&, const at::Tensor&,
     const at::Tensor&, const at::Tensor&, at::ScalarType, bool);
+// operators with their autograd nodes (autograd_ops.cpp)
+at::Tensor gelu_keep8(const at::Tensor&);
+std::tuple<at::Tensor, at::Tensor, c10::optional<at::Tensor>,
+           c10::optional<at::Tensor>>
+add_rms_norm(const at::Tensor&, const c10::optional<at::Tensor>&,
+             const at::Tensor&, double, const c10::optional<std::string>&,
+             c10::optional<at::ScalarType>);
+at::Tensor masked_linear_act(
+    const at::Tensor&, const at::Tensor&, const c10::optional<at::Tensor>&,
+    const c10::optional<at::Tensor>&, const c10::optional<at::Tensor>&,
+    const c10::optional<std::string>&, const c10::optional<at::Tensor>&,
+    c10::optional<at::ScalarType>, const c10::optional<std::string>&,
+    const c10::optional<at::Tensor>&, const c10::optional<at::Tensor>&);
 // linear layer with an epilogue (linear_act.hip)
 std::tuple<at::Tensor, c10::optional<at::Tensor>, c10::optional<at::Tensor>>
 linear_act_fwd(const at::Tensor&, const at::Tensor&,
@@ -210,4 +223,12 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         "act(x w^T + bias) + residual -> (y, kept z, its scales)");
   m.def("linear_act_bwd", &turboprune::linear_act_bwd,
         "gradients of linear_act_fwd -> (dx, dw, dbias)");
+  m.def("gelu_keep8", &turboprune::gelu_keep8,
+        "exact GELU, its input kept in 8 bits (autograd)");
+  m.def("add_rms_norm", &turboprune::add_rms_norm,
+        "(x, residual, weight, eps, keep, out_dtype) -> (y, h, codes, "
+        "scales) (autograd)");
+  m.def("masked_linear_act", &turboprune::masked_linear_act,
+        "(x, weight, mask, bias, residual, act, cache, compute_dtype, keep, "
+        "codes, scales) -> y (autograd)");
 }

@@ -19,6 +19,7 @@ from typing import Optional
 
 import torch
 import torch.nn.functional as F
+from torch.autograd.function import once_differentiable
 
 from turboprune_amd.ops import _backend
 from turboprune_amd.ops import act8
@@ -146,7 +147,8 @@ ACTS = (None, "gelu")
 
 class _MaskedLinearAct(torch.autograd.Function):
     """One node from the raw weight: product, bias, activation and residual
-    forward; dx, masked dw, db and dresidual backward."""
+    forward; dx, masked dw, db and dresidual backward. The plain form, for CPU
+    tensors; on a GPU the node is the extension's."""
 
     @staticmethod
     def forward(ctx, x, w, weight, mask, bias, residual, act, keep, codes,
@@ -156,7 +158,7 @@ class _MaskedLinearAct(torch.autograd.Function):
         need_x, need_z = need[2], need[0] or need[2] or need[4]
         if keep is not None and codes is None and need_x:
             codes, scales = act8.quantize_act8(x)
-        y, z, zs = _linear_act_fwd(
+        y, z, zs = _linear_act_fwd_plain(
             x, w, bias, residual, act,
             0 if not need_z else 1 if keep is None else 2)
         kept = (None, None) if not need_x else \
@@ -167,12 +169,13 @@ class _MaskedLinearAct(torch.autograd.Function):
         return y
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
         w, z, zs, xk, xs, mask = ctx.saved_tensors
         need = ctx.needs_input_grad
         dx = dw = db = None
         if need[0] or need[2] or need[4]:
-            dx, dw, db = _linear_act_bwd(
+            dx, dw, db = _linear_act_bwd_plain(
                 dy, z, zs, xk, xs, w, mask, need[0],
                 ctx.weight[0] if need[2] else None,
                 ctx.bias if need[4] else None)
@@ -182,10 +185,7 @@ class _MaskedLinearAct(torch.autograd.Function):
                 None, None)
 
 
-def _linear_act_fwd(x, w, bias, residual, act, keep):
-    if _backend.use_native(x, w):
-        return _backend.extension().linear_act_fwd(
-            x, w, bias, residual, act is not None, keep)
+def _linear_act_fwd_plain(x, w, bias, residual, act, keep):
     from turboprune_amd.ops.norm_act import gelu_plain
     z = x.float() @ w.float().t()
     if bias is not None:
@@ -200,10 +200,7 @@ def _linear_act_fwd(x, w, bias, residual, act, keep):
         (y, *act8.quantize_act8(z))
 
 
-def _linear_act_bwd(dy, z, zs, xk, xs, w, mask, want_dx, dw_type, db_type):
-    if _backend.use_native(dy, w):
-        return _backend.extension().linear_act_bwd(
-            dy, z, zs, xk, xs, w, mask, want_dx, dw_type, db_type)
+def _linear_act_bwd_plain(dy, z, zs, xk, xs, w, mask, want_dx, dw_type, db_type):
     from turboprune_amd.ops.norm_act import gelu_slope
     dz = dy.float()
     if z is not None:
@@ -253,6 +250,11 @@ def masked_linear_act(x: torch.Tensor, weight: torch.Tensor,
     ``add_rms_norm`` hands it on. The weight's gradient is masked and has the
     weight's type.
     """
+    if _backend.use_native(x):
+        codes, scales = kept if kept is not None else (None, None)
+        return _backend.extension().masked_linear_act(
+            x, weight, mask, bias, residual, act, cache, compute_dtype, keep,
+            codes, scales)
     act8.check_keep(keep)
     if act not in ACTS:
         raise ValueError(f"act={act!r}: one of {ACTS}")
@@ -286,11 +288,7 @@ def masked_linear_act(x: torch.Tensor, weight: torch.Tensor,
         with torch.no_grad():
             w = _masked_compute(weight, mask, ct)
     ct = w.dtype
-    if ct not in (torch.bfloat16, torch.float16) and (
-            x.is_cuda or ct != torch.float32):
-        raise TypeError("masked_linear_act computes in bfloat16 or float16 "
-                        f"on a GPU, not in {ct}: give a cache or a "
-                        "compute_dtype of such a type")
+    act8.check_float("the compute type", w)
     if residual is not None and residual.dtype not in (ct, torch.float32):
         raise TypeError(f"masked_linear_act: residual in {ct} or float32 "
                         f"expected, not {residual.dtype}")
@@ -317,7 +315,7 @@ def masked_linear_act(x: torch.Tensor, weight: torch.Tensor,
         y = _MaskedLinearAct.apply(x2, w, weight, mask, bias, r2, act, keep,
                                    codes, scales)
     else:
-        y = _linear_act_fwd(x2, w, bias, r2, act, 0)[0]
+        y = _linear_act_fwd_plain(x2, w, bias, r2, act, 0)[0]
     return y if x.dim() == 2 else y.reshape(lead + (N,))
 
 

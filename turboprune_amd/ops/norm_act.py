@@ -18,6 +18,8 @@ import torch.nn.functional as F
 
 from typing import Optional, Tuple
 
+from torch.autograd.function import once_differentiable
+
 from turboprune_amd.ops import _backend
 from turboprune_amd.ops import act8
 from turboprune_amd.ops.act8 import Act8
@@ -71,22 +73,18 @@ class _GeluFn(torch.autograd.Function):
 
 
 class _GeluKeep8Fn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x):
-        if _backend.use_native(x):
-            y, codes, scales = _backend.extension().gelu_keep8_fwd(x)
-        else:
-            y = gelu_plain(x.float()).to(x.dtype)
-            codes, scales = act8.quantize_act8(x)
-        ctx.save_for_backward(codes, scales)
-        return y
+    """The plain form, for CPU tensors; on a GPU the node is the
+    extension's."""
 
     @staticmethod
+    def forward(ctx, x):
+        ctx.save_for_backward(*act8.quantize_act8(x))
+        return gelu_plain(x.float()).to(x.dtype)
+
+    @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
-        codes, scales = ctx.saved_tensors
-        if _backend.use_native(dy):
-            return _backend.extension().gelu_keep8_bwd(codes, scales, dy)
-        z = act8.dequantize_act8(Act8(codes, scales), torch.float32)
+        z = act8.dequantize_act8(Act8(*ctx.saved_tensors), torch.float32)
         return (dy.float() * gelu_slope(z)).to(dy.dtype)
 
 
@@ -110,6 +108,8 @@ def gelu(x: torch.Tensor, keep: Optional[str] = None) -> torch.Tensor:
     act8.check_keep(keep)
     if keep is None or not (torch.is_grad_enabled() and x.requires_grad):
         return _gelu(x)
+    if _backend.use_native(x):
+        return _backend.extension().gelu_keep8(x)
     act8.check_float("x", x)
     if x.dim() < 1:
         raise ValueError("gelu(keep=...): a tensor of at least one dimension")
@@ -142,11 +142,13 @@ class FusedGELU(nn.Module):
 
 
 class _AddRMSNormFn(torch.autograd.Function):
+    """The plain form, for CPU tensors."""
+
     @staticmethod
     def forward(ctx, x, residual, weight, eps, out_dtype, keep):
         ctx.set_materialize_grads(False)
-        y, h, rstd, codes, scales = _rms_fwd(x, residual, weight, eps,
-                                             out_dtype, True, keep)
+        y, h, rstd, codes, scales = _rms_fwd_plain(x, residual, weight, eps,
+                                                   out_dtype, keep)
         ctx.save_for_backward(x if h is None else h, weight, rstd)
         ctx.x_dtype, ctx.residual = x.dtype, residual is not None
         if codes is not None:
@@ -154,25 +156,18 @@ class _AddRMSNormFn(torch.autograd.Function):
         return y, h, codes, scales
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy, dh, *_):
         h, weight, rstd = ctx.saved_tensors
         if dy is None:            # only the sum was used
             dx = None if dh is None else dh.to(ctx.x_dtype)
             return dx, dh, None, None, None, None
-        if _backend.use_native(dy):
-            dx, dr, dw = _backend.extension().rms_bwd(
-                dy, dh, h, weight, rstd, ctx.x_dtype, ctx.residual)
-        else:
-            dx, dr, dw = _rms_bwd_plain(dy, dh, h, weight, rstd,
-                                        ctx.x_dtype, ctx.residual)
+        dx, dr, dw = _rms_bwd_plain(dy, dh, h, weight, rstd, ctx.x_dtype,
+                                    ctx.residual)
         return dx, dr, dw.to(weight.dtype), None, None, None
 
 
-def _rms_fwd(x, residual, weight, eps, out_dtype, want_rstd, keep):
-    if _backend.use_native(x):
-        return _backend.extension().rms_fwd(x, residual, weight, eps,
-                                            out_dtype, want_rstd,
-                                            keep is not None)
+def _rms_fwd_plain(x, residual, weight, eps, out_dtype, keep):
     h = None if residual is None else \
         (x.float() + residual.float()).to(residual.dtype)
     hf = (x if h is None else h).float()
@@ -216,6 +211,10 @@ def add_rms_norm(x: torch.Tensor, residual: Optional[torch.Tensor],
     in any of the three types. Rows may lie at any distance. Statistics and
     the weight's gradient are summed in float32, in a fixed order.
     """
+    if _backend.use_native(x):
+        y, h, codes, scales = _backend.extension().add_rms_norm(
+            x, residual, weight, eps, keep, out_dtype)
+        return y, h, None if codes is None else Act8(codes, scales)
     act8.check_keep(keep)
     act8.check_float("x", x)
     act8.check_float("weight", weight)
@@ -249,8 +248,8 @@ def add_rms_norm(x: torch.Tensor, residual: Optional[torch.Tensor],
         y, h, codes, scales = _AddRMSNormFn.apply(x, residual, weight, eps,
                                                   out_dtype, keep)
     else:
-        y, h, _, codes, scales = _rms_fwd(x, residual, weight, eps,
-                                          out_dtype, False, keep)
+        y, h, _, codes, scales = _rms_fwd_plain(x, residual, weight, eps,
+                                                out_dtype, keep)
     return (y, x if h is None else h,
             None if codes is None else Act8(codes, scales))
 
