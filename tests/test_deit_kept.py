@@ -1,0 +1,206 @@
+"""DeiT on the fused operators: RMS norms, activations kept in 8 bits."""
+
+import pytest
+import torch
+
+from turboprune_amd.config import compose
+from turboprune_amd.config.schema import ConfigError, validate_config
+from turboprune_amd.models import build_model
+from turboprune_amd.models.deit import (DistilledVisionTransformer,
+                                        VisionTransformer)
+from turboprune_amd.ops.mask_layers import masked_modules
+
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+
+
+def vit(dev, cls=VisionTransformer, **kw):
+    torch.manual_seed(0)
+    m = cls(img_size=32, patch_size=8, embed_dim=96, depth=2, num_heads=3,
+            num_classes=10, **kw)
+    for _, layer in masked_modules(m):
+        layer.set_er_mask(0.7, seed=1)
+    return m.to(dev)
+
+
+def step(m, dev, seed=3):
+    """Loss and gradients of one step, in bfloat16 on a GPU."""
+    torch.manual_seed(seed)
+    x = torch.randn(6, 3, 32, 32).to(dev)
+    y = torch.randint(0, 10, (6,)).to(dev)
+    m.zero_grad()
+    if dev == "cuda":
+        for _, layer in masked_modules(m):
+            layer.enable_cache(torch.bfloat16)
+    with torch.autocast(device_type=dev, dtype=torch.bfloat16,
+                        enabled=dev == "cuda"):
+        loss = torch.nn.functional.cross_entropy(m(x).float(), y)
+    loss.backward()
+    return loss.item(), {n: p.grad.double().cpu()
+                         for n, p in m.named_parameters()}
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_kept_layer_norm_model_is_the_plain_one(dev):
+    plain, kept = vit(dev), vit(dev, keep="e4m3")
+    assert list(plain.state_dict()) == list(kept.state_dict())
+    kept.load_state_dict(plain.state_dict())
+    (a, ga), (b, gb) = step(plain, dev), step(kept, dev)
+    # the loss reads nothing that is kept; bf16 roundings fall elsewhere
+    assert abs(a - b) < (1e-5 if dev == "cpu" else 2e-2)
+    for n in ga:
+        # a kept value is off by 2^-4 of itself at most, 2^-5.2 in the mean
+        # square: two layers' worth of it stays below an eighth
+        assert (ga[n] - gb[n]).norm() < 2.0 ** -3 * ga[n].norm() + 1e-9, n
+    for n, layer in masked_modules(kept):
+        assert (gb[n + ".weight"].reshape(-1)[
+            layer.mask.cpu().reshape(-1) == 0] == 0).all()
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_rms_model_against_its_formulas(dev):
+    """Without keeping: the same model from elementary operations in 64
+    bits."""
+    m = vit(dev, norm="rms")
+    assert not any("norm" in k and "bias" in k for k in m.state_dict())
+    loss, grads = step(m, dev)
+    ref = vit("cpu", norm="rms").double()
+    ref.load_state_dict({k: v.cpu() for k, v in m.state_dict().items()})
+
+    def norm(mod, x):
+        return x * (x.square().mean(-1, keepdim=True) + mod.eps).rsqrt() \
+            * mod.weight
+
+    def lin(mod, x):
+        return x @ (mod.weight * mod.mask).squeeze(-1).t() + mod.bias
+    torch.manual_seed(3)
+    x = torch.randn(6, 3, 32, 32).double()
+    y = torch.randint(0, 10, (6,))
+    pe = ref.patch_embed.proj
+    t = torch.nn.functional.conv2d(x, pe.weight * pe.mask, pe.bias, 8)
+    t = t.flatten(2).transpose(1, 2)
+    t = torch.cat((ref.cls_token.expand(6, -1, -1), t), 1) + ref.pos_embed
+    for b in ref.blocks:
+        q, k, v = lin(b.attn.qkv, norm(b.norm1, t)).reshape(
+            6, 17, 3, 3, 32).permute(2, 0, 3, 1, 4)
+        p = torch.softmax(q @ k.transpose(-1, -2) * 32 ** -0.5, -1)
+        t = t + lin(b.attn.proj, (p @ v).transpose(1, 2).reshape(6, 17, 96))
+        t = t + lin(b.mlp.fc2, torch.nn.functional.gelu(
+            lin(b.mlp.fc1, norm(b.norm2, t))))
+    out = lin(ref.head, norm(ref.norm, t)[:, 0])
+    want = torch.nn.functional.cross_entropy(out, y)
+    want.backward()
+    tol = 1e-5 if dev == "cpu" else 2.0 ** -5
+    assert abs(loss - want.item()) < tol
+    for n, p in ref.named_parameters():
+        assert (grads[n] - p.grad).norm() < tol * p.grad.norm() + 1e-9, n
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_rms_kept_and_distilled(dev):
+    a, ga = step(vit(dev, norm="rms"), dev)
+    b, gb = step(vit(dev, norm="rms", keep="e4m3"), dev)
+    assert abs(a - b) < (1e-5 if dev == "cpu" else 2e-2)
+    for n in ga:
+        assert (ga[n] - gb[n]).norm() < 2.0 ** -3 * ga[n].norm() + 1e-9, n
+    m = vit(dev, DistilledVisionTransformer, norm="rms", keep="e4m3",
+            drop_rate=0.1).train()
+    if dev == "cuda":
+        for _, layer in masked_modules(m):
+            layer.enable_cache(torch.bfloat16)
+    amp = torch.autocast(device_type=dev, dtype=torch.bfloat16,
+                         enabled=dev == "cuda")
+    with amp:
+        p, q = m(torch.randn(2, 3, 32, 32, device=dev))
+    (p.float().sum() + q.float().sum()).backward()
+    assert all(v.grad is not None and v.grad.isfinite().all()
+               for v in m.parameters())
+    m.eval()
+    with torch.no_grad(), amp:
+        assert m(torch.randn(2, 3, 32, 32, device=dev)).shape == (2, 10)
+
+
+def test_config():
+    cfg = compose("imagenet_deit_lrr", ["model_params=mp_deit_small_keep8"])
+    validate_config(cfg)
+    cfg.model_params.model_name = "local_deit_tiny_patch16_224"
+    m = build_model(cfg, num_classes=10).model
+    assert m.blocks[0].keep == "e4m3"
+    assert type(m.blocks[0].norm2).__name__ == "FusedRMSNorm"
+    for over in ("+model_params.norm=batch",
+                 "+model_params.keep_activations=int8"):
+        with pytest.raises(ConfigError):
+            validate_config(compose("imagenet_deit_lrr", [over]))
+    cfg = compose("imagenet_deit_lrr", ["+model_params.norm=rms",
+                                        "model_params.model_name=resnet18"])
+    with pytest.raises(ValueError):
+        build_model(cfg)
+    for kw in ({"norm": "batch"}, {"keep": "int8"}):
+        with pytest.raises(ValueError):
+            vit("cpu", **kw)
+
+
+@pytest.mark.gpu
+def test_kept_model_needs_less_memory():
+    """Between forward and backward, of what a block's linear layers and norms
+    hold: 8-bit codes in place of 16- and 32-bit values."""
+    def live(keep):
+        m = vit("cuda", norm="rms", keep=keep)
+        for _, layer in masked_modules(m):
+            layer.enable_cache(torch.bfloat16)
+        x = torch.randn(256, 3, 32, 32, device="cuda")
+
+        def held():       # what was asked for, without the allocator's rounding
+            return torch.cuda.memory_stats()["requested_bytes.all.current"]
+        with torch.autocast("cuda", dtype=torch.bfloat16):
+            m(x[:2]).sum().backward()
+            torch.cuda.synchronize()
+            before = held()
+            y = m(x)
+            return held() - before - y.numel() * 2
+    rows = 256 * 17 * 2                          # tokens of both blocks
+    saved = live(None) - live("e4m3")
+    # inputs of qkv (96), fc1 (96) and fc2 (384) and the pre-activation (384)
+    # in 33/32 B a value against 2; proj's input (96) is the attention's own
+    # saved output, whose codes come on top
+    want = rows * ((96 * 2 + 384 * 2) * (2 - 33 / 32) - 96 * 33 / 32)
+    assert abs(saved - want) < 0.01 * want
+
+
+@pytest.mark.gpu
+def test_kept_step_in_a_graph():
+    m = vit("cuda", norm="rms", keep="e4m3")
+    for _, layer in masked_modules(m):
+        layer.enable_cache(torch.bfloat16)
+    x = torch.randn(8, 3, 32, 32, device="cuda")
+
+    def run():
+        for p in m.parameters():
+            if p.grad is not None:
+                p.grad.zero_()
+        with torch.autocast("cuda", dtype=torch.bfloat16,
+                            cache_enabled=False):
+            loss = m(x).float().square().mean()
+        loss.backward()
+        return loss
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(3):
+            run()
+    torch.cuda.current_stream().wait_stream(side)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        loss = run()
+    for seed in range(3):
+        torch.manual_seed(seed)
+        x.copy_(torch.randn_like(x))
+        g.replay()
+        torch.cuda.synchronize()
+        got = [p.grad.clone() for p in m.parameters()]
+        l0 = loss.item()
+        l1 = run().item()
+        torch.cuda.synchronize()
+        assert abs(l0 - l1) <= 2.0 ** -7 * abs(l1)
+        for a, p in zip(got, m.parameters()):
+            # library attention and reductions may take another order
+            assert (a - p.grad).norm() <= 2.0 ** -5 * p.grad.norm() + 1e-9

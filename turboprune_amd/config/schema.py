@@ -24,6 +24,8 @@ SCHEDULER_TYPES = (
 DATASETS = ("CIFAR10", "CIFAR100", "ImageNet")
 DATALOADER_TYPES = ("torch", "airbench", "ffcv", "webdataset", "synthetic", "native")
 MASK_LAYER_TYPES = ("ConvMask", "LinearMask")
+NORMS = ("layer", "rms")
+KEPT_FORMATS = ("e4m3",)
 PRECISIONS = ("bfloat16", "float16", "float32")
 CYCLIC_STRATEGIES = (
     "linear_increase", "linear_decrease", "exponential_decrease",
@@ -76,6 +78,9 @@ def validate_config(cfg: Any) -> None:
     # model_params
     _req(cfg, "model_params", "model_name", errors, str)
     _choice(cfg, "model_params", "mask_layer_type", MASK_LAYER_TYPES, errors)
+    _choice(cfg, "model_params", "norm", NORMS, errors, required=False)
+    _choice(cfg, "model_params", "keep_activations", KEPT_FORMATS, errors,
+            required=False)
 
     # pruning_params
     method = _choice(cfg, "pruning_params", "prune_method", PRUNE_METHODS, errors)

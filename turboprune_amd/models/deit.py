@@ -11,6 +11,12 @@ latent-broken. This is a working native implementation:
   custom_models.py:219) and the patch-embed conv is ``ConvMask``;
 - attention itself uses torch SDPA on ROCm; the masked qkv/proj/mlp
   projections are the MFMA masked-GEMM hot path.
+
+Two options beyond the reference, off by default, make a block run on the
+fused operators (``Block._fused``): ``norm="rms"`` takes root-mean-square
+norms that add the residual on the way, ``keep="e4m3"`` holds what the linear
+layers and the MLP's GELU need for the backward pass in 8 bits. Either way the
+bias, GELU and residual are in the products' epilogues.
 """
 
 from __future__ import annotations
@@ -20,8 +26,13 @@ from functools import partial
 import torch
 import torch.nn as nn
 
+from turboprune_amd.ops.act8 import check_keep
 from turboprune_amd.ops.mask_layers import Conv1dMask, ConvMask
-from turboprune_amd.ops.norm_act import FusedGELU, FusedLayerNorm
+from turboprune_amd.ops.norm_act import (FusedGELU, FusedLayerNorm,
+                                         FusedRMSNorm)
+
+
+NORMS = {"layer": FusedLayerNorm, "rms": FusedRMSNorm}
 
 
 class PatchEmbed(nn.Module):
@@ -76,8 +87,17 @@ class Attention(nn.Module):
         self.proj_drop = nn.Dropout(proj_drop)
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
-        B, N, C = x.shape
-        qkv = self.qkv(x).reshape(B, N, 3, self.num_heads, self.head_dim)
+        return self.proj_drop(self.proj(self._heads(self.qkv(x), x.shape)))
+
+    def fused(self, x: torch.Tensor, keep=None, kept=None) -> torch.Tensor:
+        """The same on the products with an epilogue; ``kept`` is x in 8
+        bits."""
+        x = self._heads(self.qkv.fused(x, keep=keep, kept=kept), x.shape)
+        return self.proj_drop(self.proj.fused(x, keep=keep))
+
+    def _heads(self, qkv: torch.Tensor, shape) -> torch.Tensor:
+        B, N, C = shape
+        qkv = qkv.reshape(B, N, 3, self.num_heads, self.head_dim)
         qkv = qkv.permute(2, 0, 3, 1, 4)      # 3, B, heads, N, hd
         q, k, v = qkv[0], qkv[1], qkv[2]
         drop = self.attn_drop.p if self.training else 0.0
@@ -87,8 +107,7 @@ class Attention(nn.Module):
         else:
             x = torch.nn.functional.scaled_dot_product_attention(
                 q, k, v, dropout_p=drop)
-        x = x.transpose(1, 2).reshape(B, N, C)
-        return self.proj_drop(self.proj(x))
+        return x.transpose(1, 2).reshape(B, N, C)
 
 
 class Mlp(nn.Module):
@@ -102,29 +121,56 @@ class Mlp(nn.Module):
     def forward(self, x):
         return self.drop(self.fc2(self.drop(self.act(self.fc1(x)))))
 
+    def fused(self, x, residual, keep=None, kept=None):
+        """``forward(x) + residual`` with GELU and the addition in the
+        products' epilogues; ``kept`` is x in 8 bits."""
+        x = self.drop(self.fc1.fused(x, act="gelu", keep=keep, kept=kept))
+        if self.training and self.drop.p > 0:   # dropped before it is added
+            return residual + self.drop(self.fc2.fused(x, keep=keep))
+        return self.fc2.fused(x, residual=residual, keep=keep)
+
 
 class Block(nn.Module):
     def __init__(self, dim, num_heads, mlp_ratio=4.0, qkv_bias=True,
-                 drop=0.0, attn_drop=0.0, norm_layer=nn.LayerNorm):
+                 drop=0.0, attn_drop=0.0, norm_layer=nn.LayerNorm,
+                 keep=None):
         super().__init__()
+        check_keep(keep)
+        self.keep = keep
         self.norm1 = norm_layer(dim)
         self.attn = Attention(dim, num_heads, qkv_bias, attn_drop, drop)
         self.norm2 = norm_layer(dim)
         self.mlp = Mlp(dim, int(dim * mlp_ratio), drop)
 
     def forward(self, x):
+        if self.keep is not None or isinstance(self.norm1, FusedRMSNorm):
+            return self._fused(x)
         x = x + self.attn(self.norm1(x))
         x = x + self.mlp(self.norm2(x))
         return x
+
+    def _fused(self, x):
+        keep = self.keep
+        if not isinstance(self.norm1, FusedRMSNorm):
+            x = x + self.attn.fused(self.norm1(x), keep)
+            return self.mlp.fused(self.norm2(x), x, keep)
+        # the second norm adds the attention's output to the stream; both hand
+        # their rows on in 8 bits as well, which the next product keeps
+        y, x, kept = self.norm1.add(x, None, keep)
+        y, x, kept = self.norm2.add(self.attn.fused(y, keep, kept), x, keep)
+        return self.mlp.fused(y, x, keep, kept)
 
 
 class VisionTransformer(nn.Module):
     def __init__(self, img_size=224, patch_size=16, in_chans=3,
                  num_classes=1000, embed_dim=768, depth=12, num_heads=12,
                  mlp_ratio=4.0, qkv_bias=True, drop_rate=0.0,
-                 attn_drop_rate=0.0, norm_layer=None):
+                 attn_drop_rate=0.0, norm_layer=None, norm="layer",
+                 keep=None):
         super().__init__()
-        norm_layer = norm_layer or partial(FusedLayerNorm, eps=1e-6)
+        if norm not in NORMS:
+            raise ValueError(f"norm={norm!r}: one of {tuple(NORMS)}")
+        norm_layer = norm_layer or partial(NORMS[norm], eps=1e-6)
         self.num_classes = num_classes
         self.embed_dim = embed_dim
         self.patch_embed = PatchEmbed(img_size, patch_size, in_chans, embed_dim)
@@ -135,7 +181,7 @@ class VisionTransformer(nn.Module):
         self.pos_drop = nn.Dropout(drop_rate)
         self.blocks = nn.ModuleList([
             Block(embed_dim, num_heads, mlp_ratio, qkv_bias, drop_rate,
-                  attn_drop_rate, norm_layer)
+                  attn_drop_rate, norm_layer, keep)
             for _ in range(depth)])
         self.norm = norm_layer(embed_dim)
         self.head = Conv1dMask(embed_dim, num_classes, bias=True) \
@@ -210,8 +256,7 @@ def _deit(embed_dim, depth, num_heads, img_size=224, distilled=False,
     cls = DistilledVisionTransformer if distilled else VisionTransformer
     return cls(img_size=img_size, patch_size=16, embed_dim=embed_dim,
                depth=depth, num_heads=num_heads, mlp_ratio=4.0,
-               qkv_bias=True, num_classes=num_classes,
-               norm_layer=partial(FusedLayerNorm, eps=1e-6), **kwargs)
+               qkv_bias=True, num_classes=num_classes, **kwargs)
 
 
 # factory names mirror the reference's timm registrations (utils/deit.py:69-253)

@@ -147,7 +147,9 @@ def num_classes_of(dataset_name: str) -> int:
 def build_model(cfg: Any, num_classes: Optional[int] = None) -> PruneModel:
     """Construct the masked model named by ``cfg.model_params.model_name``
     (resnet*/vgg*/local_deit_*), with CIFAR stem surgery for CIFAR
-    datasets (reference: custom_models.py:169-245, fixed DeiT path)."""
+    datasets (reference: custom_models.py:169-245, fixed DeiT path).
+    ``model_params.norm`` and ``model_params.keep_activations`` choose the
+    local_deit_* models' norm and what they keep for the backward pass."""
     name = cfg.model_params.model_name
     dataset = cfg.dataset_params.dataset_name
     if num_classes is None:
@@ -170,5 +172,12 @@ def build_model(cfg: Any, num_classes: Optional[int] = None) -> PruneModel:
     kwargs = {"num_classes": num_classes}
     if name.startswith(("resnet", "vgg")):
         kwargs["cifar_stem"] = dataset in ("CIFAR10", "CIFAR100")
+    for key, arg in (("norm", "norm"), ("keep_activations", "keep")):
+        value = cfg.select(f"model_params.{key}", None)
+        if value is not None:
+            if not name.startswith("local_deit"):
+                raise ValueError(f"model_params.{key} is for the local_deit_* "
+                                 f"models, not {name}")
+            kwargs[arg] = value
     inner = factory(**kwargs)
     return PruneModel(inner)

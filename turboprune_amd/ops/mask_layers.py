@@ -87,6 +87,13 @@ class _MaskedMixin:
         else:
             self.weight_masked = wm
 
+    def _fused_dtype(self, x: torch.Tensor) -> Optional[torch.dtype]:
+        """The type that a product without a cache computes in."""
+        if self.compute_dtype is None and torch.is_autocast_enabled(
+                x.device.type):
+            return torch.get_autocast_dtype(x.device.type)
+        return self.compute_dtype
+
     def _load_from_state_dict(self, *args, **kwargs):
         super()._load_from_state_dict(*args, **kwargs)
         self.refresh_cache()
@@ -185,7 +192,7 @@ class LinearMask(_MaskedMixin, nn.Linear):
         backward pass needs in 8 bits."""
         return TF.masked_linear_act(
             x, self.weight, self.mask, self.bias, residual, act,
-            self._fresh_cache(), self.compute_dtype, keep, kept)
+            self._fresh_cache(), self._fused_dtype(x), keep, kept)
 
 
 class Conv1dMask(_MaskedMixin, nn.Conv1d):
@@ -214,7 +221,7 @@ class Conv1dMask(_MaskedMixin, nn.Conv1d):
         return TF.masked_linear_act(
             x, self.weight.squeeze(-1), self.mask.squeeze(-1), self.bias,
             residual, act, cache.squeeze(-1) if cache is not None else None,
-            self.compute_dtype, keep, kept)
+            self._fused_dtype(x), keep, kept)
 
 
 MASKED_LAYER_TYPES = (ConvMask, LinearMask, Conv1dMask)
