@@ -74,7 +74,7 @@ def kept_z(d, t, act, keep, compute):
     if x.is_cuda:
         from turboprune_amd.ops._backend import extension
         return extension().linear_act_fwd(x, w, bias, None, True,
-                                          2 if keep else 1)[1:]
+                                          2 if keep else 1, False)[1:3]
     return TF._linear_act_fwd_plain(x, w, bias, None, "gelu",
                                     2 if keep else 1)[1:]
 
@@ -416,12 +416,14 @@ def test_refusals_on_the_gpu():
     ext = extension()
     xb, wb = x.bfloat16(), w.cuda().bfloat16()
     for bad in (lambda: ext.linear_act_fwd(xb, wb[:, :8], None, None, False,
-                                           0),
+                                           0, False),
                 lambda: ext.linear_act_fwd(xb, wb.half(), None, None, False,
-                                           0),
-                lambda: ext.linear_act_fwd(xb, wb, m[0], None, False, 0),
-                lambda: ext.linear_act_fwd(xb, wb, None, xb, False, 0),
-                lambda: ext.linear_act_fwd(xb[:0], wb, None, None, False, 0),
+                                           0, False),
+                lambda: ext.linear_act_fwd(xb, wb, m[0], None, False, 0,
+                                           False),
+                lambda: ext.linear_act_fwd(xb, wb, None, xb, False, 0, False),
+                lambda: ext.linear_act_fwd(xb[:0], wb, None, None, False, 0,
+                                           False),
                 lambda: ext.linear_act_bwd(xb, None, None, xb, None, wb,
                                            None, True, None, None),
                 lambda: ext.linear_act_bwd(
@@ -451,6 +453,28 @@ def test_layers(dev, cls):
     assert (layer.weight.grad[layer.mask == 0] == 0).all()
     assert layer.weight.grad.dtype == F32
     assert layer.bias.grad.shape == (48,)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t", [BF16, FP16])
+@pytest.mark.parametrize("M,K,N", [
+    (1, 8, 8), (3, 33, 47), (65, 200, 300), (130, 1000, 700), (70, 64, 2000),
+    (5000, 384, 1000), (20000, 72, 400), (52000, 520, 256)])
+def test_input_kept_by_the_product(t, M, K, N):
+    """The codes that the product writes of its input are quantise_act8's, in
+    each of the tile sizes."""
+    from turboprune_amd.ops._backend import extension
+    d = make(M, K, N, t, None, "cuda")
+    x = d["x"] * torch.exp2(torch.randint(-9, 9, (M, 1), device="cuda")).to(t)
+    x[M // 2, K // 3] = float("nan")
+    x[M // 3, K // 2] = float("inf")
+    _, _, _, c, s = extension().linear_act_fwd(
+        x, d["weight"].to(t), None, None, False, 0, True)
+    ref = quantize_act8(x)
+    assert torch.equal(c.view(torch.uint8) & 127,
+                       ref.codes.view(torch.uint8) & 127)
+    assert torch.equal(c.float().nan_to_num(0), ref.codes.float().nan_to_num(0))
+    assert torch.equal(s.view(torch.uint8), ref.scales.view(torch.uint8))
 
 
 @pytest.mark.gpu

@@ -49,24 +49,27 @@ TP_DEVICE void load8<float>(const float* p, float (&v)[8]) {
     v[i + 4] = __uint_as_float(b[i]);
   }
 }
-template <>
-TP_DEVICE void load8<__hip_bfloat16>(const __hip_bfloat16* p, float (&v)[8]) {
-  u32x4 d = *reinterpret_cast<const u32x4_a2*>(p);
+template <typename T>
+TP_DEVICE void unpack8(u32x4 d, float (&v)[8]) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    v[2 * i] = __uint_as_float(d[i] << 16);
-    v[2 * i + 1] = __uint_as_float(d[i] & 0xffff0000u);
+    if constexpr (__is_same(T, _Float16)) {
+      f16x2v e = __builtin_bit_cast(f16x2v, (uint32_t)d[i]);
+      v[2 * i] = (float)e[0];
+      v[2 * i + 1] = (float)e[1];
+    } else {
+      v[2 * i] = __uint_as_float(d[i] << 16);
+      v[2 * i + 1] = __uint_as_float(d[i] & 0xffff0000u);
+    }
   }
 }
 template <>
+TP_DEVICE void load8<__hip_bfloat16>(const __hip_bfloat16* p, float (&v)[8]) {
+  unpack8<__hip_bfloat16>(*reinterpret_cast<const u32x4_a2*>(p), v);
+}
+template <>
 TP_DEVICE void load8<_Float16>(const _Float16* p, float (&v)[8]) {
-  u32x4 d = *reinterpret_cast<const u32x4_a2*>(p);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    f16x2v e = __builtin_bit_cast(f16x2v, (uint32_t)d[i]);
-    v[2 * i] = (float)e[0];
-    v[2 * i + 1] = (float)e[1];
-  }
+  unpack8<_Float16>(*reinterpret_cast<const u32x4_a2*>(p), v);
 }
 
 // two floats to two packed 16-bit values, each rounded to nearest even

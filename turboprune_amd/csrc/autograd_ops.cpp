@@ -13,7 +13,6 @@ using torch::autograd::variable_list;
 using OptTensor = c10::optional<at::Tensor>;
 
 at::Tensor mask_apply(const at::Tensor&, const at::Tensor&, at::ScalarType);
-std::tuple<at::Tensor, at::Tensor> act8_quantize(const at::Tensor&);
 std::tuple<at::Tensor, at::Tensor, at::Tensor> gelu_keep8_fwd(
     const at::Tensor&);
 at::Tensor gelu_keep8_bwd(const at::Tensor&, const at::Tensor&,
@@ -24,9 +23,9 @@ std::tuple<at::Tensor, OptTensor, OptTensor, OptTensor, OptTensor> rms_fwd(
 std::tuple<at::Tensor, OptTensor, at::Tensor> rms_bwd(
     const at::Tensor&, const OptTensor&, const at::Tensor&, const at::Tensor&,
     const at::Tensor&, at::ScalarType, bool);
-std::tuple<at::Tensor, OptTensor, OptTensor> linear_act_fwd(
-    const at::Tensor&, const at::Tensor&, const OptTensor&, const OptTensor&,
-    bool, int64_t);
+std::tuple<at::Tensor, OptTensor, OptTensor, OptTensor, OptTensor>
+linear_act_fwd(const at::Tensor&, const at::Tensor&, const OptTensor&,
+               const OptTensor&, bool, int64_t, bool);
 std::tuple<OptTensor, OptTensor, OptTensor> linear_act_bwd(
     const at::Tensor&, const OptTensor&, const OptTensor&, const OptTensor&,
     const OptTensor&, const at::Tensor&, const OptTensor&, bool,
@@ -145,18 +144,19 @@ struct LinearAct : Function<LinearAct> {
     bool need_b = bias && bias->requires_grad();
     bool need_z = x.requires_grad() || need_x || need_b;   // for the slope
     at::Tensor codes, scales;
-    if (keep && need_x) {
-      if (codes_in) {
-        codes = codes_in->reshape(x2.sizes());
-        scales = scales_in->reshape({x2.size(0), -1});
-      } else {
-        std::tie(codes, scales) = act8_quantize(x2);
-      }
+    if (keep && need_x && codes_in) {
+      codes = codes_in->reshape(x2.sizes());
+      scales = scales_in->reshape({x2.size(0), -1});
     }
     OptTensor r2;
     if (residual) r2 = residual->reshape({-1, N});
-    auto [y, z, zs] = linear_act_fwd(x2, w, bias, r2, act,
-                                     !need_z ? 0 : keep ? 2 : 1);
+    auto [y, z, zs, xc, xs] =
+        linear_act_fwd(x2, w, bias, r2, act, !need_z ? 0 : keep ? 2 : 1,
+                       keep && need_x && !codes_in);
+    if (xc) {
+      codes = *xc;
+      scales = *xs;
+    }
     ctx->save_for_backward(
         {w, or_none(z), or_none(zs),
          !need_x ? at::Tensor() : keep ? codes : x, scales,
@@ -348,7 +348,7 @@ at::Tensor masked_linear_act(
         x.dim() == 2 ? x : x.reshape({-1, K}), w, as_opt(bias),
         r.defined() ? OptTensor(r.dim() == 2 ? r : r.reshape({-1, N}))
                     : OptTensor(),
-        act, 0);
+        act, 0, false);
     return x.dim() == 2 ? std::get<0>(o) : std::get<0>(o).view(out_sizes);
   }
   return LinearAct::apply(x, w, weight, mask, as_opt(bias), residual, act,

@@ -112,10 +112,11 @@ at::Tensor masked_linear_act(
     c10::optional<at::ScalarType>, const c10::optional<std::string>&,
     const c10::optional<at::Tensor>&, const c10::optional<at::Tensor>&);
 // linear layer with an epilogue (linear_act.hip)
-std::tuple<at::Tensor, c10::optional<at::Tensor>, c10::optional<at::Tensor>>
+std::tuple<at::Tensor, c10::optional<at::Tensor>, c10::optional<at::Tensor>,
+           c10::optional<at::Tensor>, c10::optional<at::Tensor>>
 linear_act_fwd(const at::Tensor&, const at::Tensor&,
                const c10::optional<at::Tensor>&,
-               const c10::optional<at::Tensor>&, bool, int64_t);
+               const c10::optional<at::Tensor>&, bool, int64_t, bool);
 std::tuple<c10::optional<at::Tensor>, c10::optional<at::Tensor>,
            c10::optional<at::Tensor>>
 linear_act_bwd(const at::Tensor&, const c10::optional<at::Tensor>&,
@@ -220,7 +221,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("rms_bwd", &turboprune::rms_bwd,
         "RMS norm gradient -> (dx, dresidual, dweight)");
   m.def("linear_act_fwd", &turboprune::linear_act_fwd,
-        "act(x w^T + bias) + residual -> (y, kept z, its scales)");
+        "act(x w^T + bias) + residual -> (y, kept z, its scales, kept x, "
+        "its scales)");
   m.def("linear_act_bwd", &turboprune::linear_act_bwd,
         "gradients of linear_act_fwd -> (dx, dw, dbias)");
   m.def("gelu_keep8", &turboprune::gelu_keep8,

@@ -67,6 +67,7 @@ struct Mm {
   int64_t ldq, ldp;      // row distance in bytes
   int nq, np;            // rows (kRowK) or columns (kColK) that can be read
   const uint8_t* pscale; // kCodes: a scale for every 32 codes of a row
+  uint8_t *qcodes, *qscale;   // kRowK: Q in 8 bits, to be written, or null
   int M, N, K;           // rows and columns of C, length of the sum
   int tiles_n, tiles;    // tile grid
   int ksplit, kper;      // k-tiles of one slab; slab s writes out + s M N
@@ -224,6 +225,32 @@ struct CodeTile {
   }
 };
 
+// Q's values of one k-tile, from LDS, in 8 bits. The column tiles of a row of
+// tiles take the k-tiles in turn, so that each of them does its share and the
+// input is read once for product and codes (a pass of its own over 50432 x
+// 1536 values takes 42 us).
+template <typename T, int BQ, int BK, int THREADS>
+TP_DEVICE void keep_tile(TP_LDS const char* t, const Mm& a, int m0, int kt) {
+  constexpr int C = BK / 8;
+  static_assert(BQ * C % THREADS == 0, "whole rounds");
+#pragma unroll
+  for (int i = 0; i < BQ * C / THREADS; ++i) {
+    int at = i * THREADS + threadIdx.x, r = at / C, c = at % C;
+    u32x4 d = *reinterpret_cast<TP_LDS const u32x4*>(
+        t + r * (BK * 2) + (c ^ Tile<BQ, BK, false>::swap(r)) * 16);
+    float v[8];
+    unpack8<T>(d, v);
+    int e, col = kt * BK + c * 8;
+    uint2 q = encode8(v, e, QuadMax());
+    int64_t row = m0 + r;
+    int n = row < a.M ? a.K - col : 0;
+    if (n <= 0) continue;
+    store_codes(a.qcodes + row * a.K + col, n, q);
+    if ((c & 3) == 0)
+      a.qscale[row * ((a.K + 31) / 32) + col / 32] = (uint8_t)(e + 127);
+  }
+}
+
 template <int N>
 TP_DEVICE void wait_and_meet() {
   // this wave's loads but the newest N have landed and its reads are done;
@@ -380,6 +407,9 @@ __global__ __launch_bounds__(WQ * WP * 64, MINW) void mm_kernel(Mm a) {
       if (kt + 2 < kt1) ct.load(a, n0, kt + 2);
     }
     TP_LDS const char* b = place(kt);
+    if constexpr (QF == kRowK && PF == kRowK)
+      if (a.qcodes && kt % a.tiles_n == wg % a.tiles_n)
+        keep_tile<T, BQ, BK, NW * 64>(b, a, m0, kt);
 #pragma unroll
     for (int ks = 0; ks < BK / 32; ++ks) {
       s16x8 fq[MI], fp[NI];
@@ -642,17 +672,21 @@ int64_t tiles_of(const Mm& a, int q, int p) {
 }
 
 // Both operands along the sum. 256 x 256 by 16 waves moves the fewest bytes
-// into LDS per product but needs about a CU each to pay: 50432x1536x384 in 92
-// us against 111 with 128 x 128, but 12608x1536x384 (300 tiles, two rounds for
-// little more than one) 32 against 26. Short products end soonest in many
-// small tiles: 1576x768x768 10.2 us in 64 x 64, 12.0 in 128 x 128;
+// into LDS per product, but it needs about a CU each to pay, little of the last
+// column tile empty, and it ends with an epilogue that no other block's product
+// hides: 50432x1536x384 in 92 us against 105 with 128 x 128, 25216x1024x4096
+// in 214 against 258; but 50432x384x1536 with a 32-bit residual (a third of
+// the columns empty) in 138 against 116, 12608x1536x384 (300 tiles, two rounds
+// for little more than one) in 32 against 26. Short products end soonest in
+// many small tiles: 1576x768x768 10.2 us in 64 x 64, 12.0 in 128 x 128;
 // 3152x1536x384 (1200 small tiles) 13.8 against 12.9.
 template <typename T, int ACT>
 void run_rows(const Mm& a) {
   if (tiles_of(a, 64, 64) <= 600)
     return launch_mm<T, 64, 64, 64, 2, 2, kRowK, kRowK, 2, 1, ACT>(a);
   int64_t t = tiles_of(a, 256, 256);
-  if (t >= 200 && (a.K >= 512 || t >= 768))
+  bool filled = (a.N + 255) / 256 * 256 <= a.N + a.N / 5;
+  if (filled && t >= 200 && (a.K >= 512 || t >= 768))
     return launch_mm<T, 256, 256, 64, 4, 4, kRowK, kRowK, 2, 4, ACT>(a);
   launch_mm<T, 128, 128, 64, 2, 4, kRowK, kRowK, 2, 2, ACT>(a);
 }
@@ -687,7 +721,7 @@ void run_cols(const Mm& a, Split s) {
       return launch_mm<T, 256, 256, 64, 4, 4, kColK, PF, 2, 4>(a, s.slabs);
   }
   if (s.tile == 128)
-    return launch_mm<T, 128, 128, 64, 2, 2, kColK, PF, 2, 2>(a, s.slabs);
+    return launch_mm<T, 128, 128, 64, 2, 4, kColK, PF, 2, 2>(a, s.slabs);
   launch_mm<T, 64, 64, 64, 2, 2, kColK, PF, 2, 1>(a, s.slabs);
 }
 
@@ -698,13 +732,14 @@ void check_size(int64_t M, int64_t N, int64_t K) {
 
 }  // namespace
 
-// (y, z, scales of z). keep: 0 keeps nothing, 1 the pre-activation in 16
-// bits, 2 in 8 bits (only with act).
-std::tuple<at::Tensor, c10::optional<at::Tensor>, c10::optional<at::Tensor>>
+// (y, z, scales of z, x's codes, their scales). keep: 0 keeps nothing, 1 the
+// pre-activation in 16 bits, 2 in 8 bits (only with act); keep_x: x in 8 bits.
+std::tuple<at::Tensor, c10::optional<at::Tensor>, c10::optional<at::Tensor>,
+           c10::optional<at::Tensor>, c10::optional<at::Tensor>>
 linear_act_fwd(const at::Tensor& x, const at::Tensor& w,
                const c10::optional<at::Tensor>& bias,
                const c10::optional<at::Tensor>& residual, bool act,
-               int64_t keep) {
+               int64_t keep, bool keep_x) {
   TORCH_CHECK(x.is_cuda() && x.dim() == 2 && w.dim() == 2 &&
                   x.size(1) == w.size(1) && x.size(0) > 0 && x.size(1) > 0 &&
                   w.size(0) > 0,
@@ -746,6 +781,12 @@ linear_act_fwd(const at::Tensor& x, const at::Tensor& w,
   c10::optional<at::Tensor> z, zs;
   if (act && keep == 1) z = at::empty({M, N}, x.options());
   if (act && keep == 2) std::tie(z, zs) = act8_empty({M, N}, x.options());
+  c10::optional<at::Tensor> xc, xs;
+  if (keep_x) {
+    std::tie(xc, xs) = act8_empty({M, K}, x.options());
+    a.qcodes = (uint8_t*)xc->data_ptr();
+    a.qscale = (uint8_t*)xs->data_ptr();
+  }
   if (z) a.e.z = z->data_ptr();
   if (zs) a.e.zscale = (uint8_t*)zs->data_ptr();
   a.e.out = y.data_ptr();
@@ -766,7 +807,7 @@ linear_act_fwd(const at::Tensor& x, const at::Tensor& w,
     else
       run_rows<T, kGelu>(a);
   });
-  return {y, z, zs};
+  return {y, z, zs, xc, xs};
 }
 
 // (dx, dw, db), each only where asked for. z: the kept pre-activation (16-bit
