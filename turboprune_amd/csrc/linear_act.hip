@@ -462,6 +462,103 @@ __global__ __launch_bounds__(WQ * WP * 64, MINW) void mm_kernel(Mm a) {
     finish(std::false_type());
 }
 
+// Few rows (single tokens, a classifier's batch): the weight is read once and
+// nothing is used twice, so there are no tiles to stage. A block takes 32
+// columns; its 8 waves take 32 values of k each in turn, straight from global
+// memory into fragments (rows at any address), and their sums meet in LDS, wave
+// j finishing 16 rows. 8 columns of blocks would leave most CUs idle at 64
+// tiles of the staged kernel: 29x2875x768 takes 5 us here and 17 there.
+template <typename T>
+TP_DEVICE s16x8 frag_of(const T* p, int n) {   // n values exist
+  u32x4 d = {};
+  if (n >= 8) {
+    d = *reinterpret_cast<const u32x4_a2*>(p);
+  } else if (n > 0) {
+    const uint16_t* h = reinterpret_cast<const uint16_t*>(p);
+#pragma unroll
+    for (int i = 0; i < 7; ++i)
+      if (i < n) d[i / 2] |= (uint32_t)h[i] << (16 * (i & 1));
+  }
+  return __builtin_bit_cast(s16x8, d);
+}
+
+template <typename T, int MI, int ACT>
+__global__ __launch_bounds__(512) void rows_kernel(Mm a) {
+  constexpr int NW = 8, U = 4;   // waves; steps of k in flight
+  __shared__ f32x4 part[NW][2 * MI][64];
+  int lane = threadIdx.x & 63, g = lane >> 4;
+  int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  int n0 = blockIdx.x * 32;
+  const T* q[MI];
+  const T* p[2];
+  int nq[MI], np[2];   // values of these rows: K, or none
+#pragma unroll
+  for (int j = 0; j < MI; ++j) {
+    int row = j * 16 + (lane & 15);
+    nq[j] = row < a.M ? a.K : 0;
+    q[j] = (const T*)(a.q + (int64_t)row * a.ldq);
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    int col = n0 + i * 16 + (lane & 15);
+    np[i] = col < a.N ? a.K : 0;
+    p[i] = (const T*)(a.p + (int64_t)col * a.ldp);
+  }
+  f32x4 acc[2][MI] = {};
+  for (int k0 = wave * 32 + g * 8; k0 - g * 8 < a.K; k0 += NW * 32 * U) {
+    s16x8 fq[U][MI], fp[U][2];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      int k = k0 + u * NW * 32;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) fp[u][i] = frag_of(p[i] + k, np[i] - k);
+#pragma unroll
+      for (int j = 0; j < MI; ++j) fq[u][j] = frag_of(q[j] + k, nq[j] - k);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < MI; ++j)
+          acc[i][j] = mma<T>(fp[u][i], fq[u][j], acc[i][j]);
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < MI; ++j) part[wave][i * MI + j][lane] = acc[i][j];
+  __syncthreads();
+  if (wave >= MI) return;
+  int j = wave, row = j * 16 + (lane & 15);
+  f32x4 s[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    s[i] = part[0][i * MI + j][lane];
+#pragma unroll
+    for (int w = 1; w < NW; ++w) s[i] += part[w][i * MI + j][lane];
+    int col = n0 + i * 16 + g * 4;
+    if (a.e.bias)
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (col + k < a.N)
+          s[i][k] += a.e.bias_f32 ? ((const float*)a.e.bias)[col + k]
+                                  : to_float<T>(((const T*)a.e.bias)[col + k]);
+  }
+  float v[8];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    auto t = __builtin_amdgcn_permlane16_swap(
+        __float_as_uint(s[0][k]), __float_as_uint(s[1][k]), false, false);
+    v[k] = __uint_as_float(t[0]);
+    v[4 + k] = __uint_as_float(t[1]);
+  }
+  int c0 = n0 + (g & 1) * 16 + (g >> 1) * 8;
+  epilogue8<T, ACT, false>(
+      a.e, (int64_t)row * a.N + c0,
+      (int64_t)row * ((a.N + 31) / 32) + blockIdx.x,
+      row < a.M ? a.N - c0 : 0, g == 0, v);
+}
+
 // sum of the slabs of a split product, masked and rounded
 template <typename T>
 __global__ __launch_bounds__(kBlock) void join_kernel(
@@ -681,6 +778,19 @@ int64_t tiles_of(const Mm& a, int q, int p) {
 // many small tiles: 1576x768x768 10.2 us in 64 x 64, 12.0 in 128 x 128;
 // 3152x1536x384 (1200 small tiles) 13.8 against 12.9.
 template <typename T, int ACT>
+void run_few(const Mm& a) {
+  unsigned grid = (unsigned)((a.N + 31) / 32);
+  auto s = current();
+  if (a.M <= 16)
+    rows_kernel<T, 1, ACT><<<grid, 512, 0, s>>>(a);
+  else if (a.M <= 32)
+    rows_kernel<T, 2, ACT><<<grid, 512, 0, s>>>(a);
+  else
+    rows_kernel<T, 4, ACT><<<grid, 512, 0, s>>>(a);
+  C10_HIP_KERNEL_LAUNCH_CHECK();
+}
+
+template <typename T, int ACT>
 void run_rows(const Mm& a) {
   if (tiles_of(a, 64, 64) <= 600)
     return launch_mm<T, 64, 64, 64, 2, 2, kRowK, kRowK, 2, 1, ACT>(a);
@@ -776,7 +886,14 @@ linear_act_fwd(const at::Tensor& x, const at::Tensor& w,
     a.e.res_f32 = r.scalar_type() == at::kFloat;
     ot = r.scalar_type();
   }
-  auto xl = loadable(x), wl = loadable(w);
+  // few rows without a backward pass to come (in training every sum is the
+  // tiles', so that it does not go by what is kept); they need neither
+  // alignment nor padding
+  bool few = M <= 64 && keep == 0 && !keep_x;
+  auto in_rows = [](const at::Tensor& t) {
+    return t.size(1) <= 1 || t.stride(1) == 1 ? t : t.contiguous();
+  };
+  auto xl = few ? in_rows(x) : loadable(x), wl = few ? in_rows(w) : loadable(w);
   auto y = at::empty({M, N}, x.options().dtype(ot));
   c10::optional<at::Tensor> z, zs;
   if (act && keep == 1) z = at::empty({M, N}, x.options());
@@ -800,7 +917,9 @@ linear_act_fwd(const at::Tensor& x, const at::Tensor& w,
   a.K = (int)K;
   by16(st, [&](auto t) {
     using T = decltype(t);
-    if (!act)
+    if (few)
+      act ? run_few<T, kGelu>(a) : run_few<T, kNoAct>(a);
+    else if (!act)
       run_rows<T, kNoAct>(a);
     else if (zs)
       run_rows<T, kGelu8>(a);
