@@ -466,62 +466,97 @@ __global__ __launch_bounds__(WQ * WP * 64, MINW) void mm_kernel(Mm a) {
 // nothing is used twice, so there are no tiles to stage. A block takes 32
 // columns; its 8 waves take 32 values of k each in turn, straight from global
 // memory into fragments (rows at any address), and their sums meet in LDS, wave
-// j finishing 16 rows. 8 columns of blocks would leave most CUs idle at 64
-// tiles of the staged kernel: 29x2875x768 takes 5 us here and 17 there.
-template <typename T>
-TP_DEVICE s16x8 frag_of(const T* p, int n) {   // n values exist
-  u32x4 d = {};
-  if (n >= 8) {
-    d = *reinterpret_cast<const u32x4_a2*>(p);
-  } else if (n > 0) {
-    const uint16_t* h = reinterpret_cast<const uint16_t*>(p);
-#pragma unroll
-    for (int i = 0; i < 7; ++i)
-      if (i < n) d[i / 2] |= (uint32_t)h[i] << (16 * (i & 1));
+// j finishing 16 rows. The staged kernel would give 29x2875x768 to 12 CUs.
+//
+// 8 values of a row from p on. Where rows have an odd length they start between
+// two dwords every other time, and a 16-byte load there is taken apart by the
+// memory pipe: such lanes load the five dwords around their values and shift
+// (29x2875x768: 17 us, 27 with loads at odd addresses; 12 where K is even).
+template <typename T, bool ODD>
+struct Few {
+  u32x4 d;
+  uint32_t e, odd;
+  TP_DEVICE void load(const T* p) {   // ODD: needs two values behind the eight
+    odd = ODD ? (uint32_t)(uintptr_t)p & 2 : 0;
+    const char* c = (const char*)p - odd;
+    d = *reinterpret_cast<const u32x4_a4*>(c);
+    if constexpr (ODD) e = *reinterpret_cast<const uint32_t*>(c + 16);
   }
+  TP_DEVICE s16x8 get() const {
+    if constexpr (!ODD) return __builtin_bit_cast(s16x8, d);
+    u32x4 r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      r[i] = __builtin_amdgcn_alignbyte(i < 3 ? d[i + 1] : e, d[i], odd);
+    return __builtin_bit_cast(s16x8, r);
+  }
+};
+// the end of a row: n of 8 values exist (none where n <= 0)
+template <typename T>
+TP_DEVICE s16x8 last_of(const T* p, int n) {
+  const uint16_t* h = reinterpret_cast<const uint16_t*>(p);
+  u32x4 d = {};
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (i < n) d[i / 2] |= (uint32_t)h[i] << (16 * (i & 1));
   return __builtin_bit_cast(s16x8, d);
 }
 
-template <typename T, int MI, int ACT>
+template <typename T, int MI, int ACT, bool ODD>
 __global__ __launch_bounds__(512) void rows_kernel(Mm a) {
   constexpr int NW = 8, U = 4;   // waves; steps of k in flight
   __shared__ f32x4 part[NW][2 * MI][64];
   int lane = threadIdx.x & 63, g = lane >> 4;
   int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   int n0 = blockIdx.x * 32;
+  // rows behind the last are the last one again: what they give is not stored
   const T* q[MI];
   const T* p[2];
-  int nq[MI], np[2];   // values of these rows: K, or none
 #pragma unroll
-  for (int j = 0; j < MI; ++j) {
-    int row = j * 16 + (lane & 15);
-    nq[j] = row < a.M ? a.K : 0;
-    q[j] = (const T*)(a.q + (int64_t)row * a.ldq);
-  }
+  for (int j = 0; j < MI; ++j)
+    q[j] = (const T*)(a.q + min(j * 16 + (lane & 15), a.M - 1) * a.ldq);
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    int col = n0 + i * 16 + (lane & 15);
-    np[i] = col < a.N ? a.K : 0;
-    p[i] = (const T*)(a.p + (int64_t)col * a.ldp);
-  }
+  for (int i = 0; i < 2; ++i)
+    p[i] = (const T*)(a.p + min(n0 + i * 16 + (lane & 15), a.N - 1) * a.ldp);
   f32x4 acc[2][MI] = {};
-  for (int k0 = wave * 32 + g * 8; k0 - g * 8 < a.K; k0 += NW * 32 * U) {
-    s16x8 fq[U][MI], fp[U][2];
+  // whole steps: with ODD those that have two values behind them
+  constexpr int W = ODD ? 34 : 32;
+  int whole = a.K >= W ? (a.K - W) / 32 + 1 : 0;
+  for (int s = wave; s < whole; s += NW * U) {
+    Few<T, ODD> fq[U][MI], fp[U][2];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      int k = k0 + u * NW * 32;
+      if (s + u * NW >= whole) break;
+      int k = (s + u * NW) * 32 + g * 8;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) fp[u][i] = frag_of(p[i] + k, np[i] - k);
+      for (int i = 0; i < 2; ++i) fp[u][i].load(p[i] + k);
 #pragma unroll
-      for (int j = 0; j < MI; ++j) fq[u][j] = frag_of(q[j] + k, nq[j] - k);
+      for (int j = 0; j < MI; ++j) fq[u][j].load(q[j] + k);
     }
 #pragma unroll
-    for (int u = 0; u < U; ++u)
+    for (int u = 0; u < U; ++u) {
+      if (s + u * NW >= whole) break;
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int j = 0; j < MI; ++j)
-          acc[i][j] = mma<T>(fp[u][i], fq[u][j], acc[i][j]);
+          acc[i][j] = mma<T>(fp[u][i].get(), fq[u][j].get(), acc[i][j]);
+    }
+  }
+  // the one or two steps that end the rows
+  for (int s = whole; s * 32 < a.K; ++s) {
+    if (s % NW != wave) continue;
+    int k = s * 32 + g * 8;
+    s16x8 wq[MI], wp[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) wp[i] = last_of(p[i] + k, a.K - k);
+#pragma unroll
+    for (int j = 0; j < MI; ++j) wq[j] = last_of(q[j] + k, a.K - k);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < MI; ++j)
+        acc[i][j] = mma<T>(wp[i], wq[j], acc[i][j]);
   }
 #pragma unroll
   for (int i = 0; i < 2; ++i)
@@ -780,14 +815,21 @@ int64_t tiles_of(const Mm& a, int q, int p) {
 template <typename T, int ACT>
 void run_few(const Mm& a) {
   unsigned grid = (unsigned)((a.N + 31) / 32);
-  auto s = current();
-  if (a.M <= 16)
-    rows_kernel<T, 1, ACT><<<grid, 512, 0, s>>>(a);
-  else if (a.M <= 32)
-    rows_kernel<T, 2, ACT><<<grid, 512, 0, s>>>(a);
+  auto run = [&](auto odd) {
+    constexpr bool ODD = decltype(odd)::value;
+    auto s = current();
+    if (a.M <= 16)
+      rows_kernel<T, 1, ACT, ODD><<<grid, 512, 0, s>>>(a);
+    else if (a.M <= 32)
+      rows_kernel<T, 2, ACT, ODD><<<grid, 512, 0, s>>>(a);
+    else
+      rows_kernel<T, 4, ACT, ODD><<<grid, 512, 0, s>>>(a);
+    C10_HIP_KERNEL_LAUNCH_CHECK();
+  };
+  if (((uintptr_t)a.q | (uintptr_t)a.p | a.ldq | a.ldp) & 2)
+    run(std::true_type());
   else
-    rows_kernel<T, 4, ACT><<<grid, 512, 0, s>>>(a);
-  C10_HIP_KERNEL_LAUNCH_CHECK();
+    run(std::false_type());
 }
 
 template <typename T, int ACT>
