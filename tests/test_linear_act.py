@@ -223,6 +223,50 @@ def test_strides_and_leading_dimensions(dev):
 
 
 @pytest.mark.parametrize("dev", DEVICES)
+def test_unusual_arguments(dev):
+    """A vector for x, a weight in columns, x as its own residual, a cache
+    that asks for gradients, kept rows cut from a larger tensor, a fp16 weight
+    under a bf16 product."""
+    d = make(1, 40, 24, BF16, F32, dev)
+    ref = check(d, BF16, "gelu", "e4m3").detach()
+    v = {k: t.reshape(-1) if k in ("x", "residual", "dy") else t
+         for k, t in d.items()}
+    assert torch.equal(check(v, BF16, "gelu", "e4m3"), ref.reshape(-1))
+    d = make(30, 48, 56, BF16, BF16, dev)
+    ref = check(d, BF16, "gelu").detach()
+    cols = dict(d, weight=d["weight"].t().contiguous().t(),
+                mask=d["mask"].t().contiguous().t())
+    assert torch.equal(check(cols, BF16, "gelu"), ref)
+    d = make(30, 48, 48, BF16, BF16, dev)
+    x = d["x"].clone().requires_grad_()
+    y = TF.masked_linear_act(x, d["weight"], d["mask"], residual=x,
+                             compute_dtype=BF16)
+    g, = torch.autograd.grad(y, x, d["dy"])
+    two = d["x"].clone().requires_grad_()
+    y2 = TF.masked_linear_act(two, d["weight"], d["mask"],
+                              residual=d["x"], compute_dtype=BF16)
+    h, = torch.autograd.grad(y2, two, d["dy"])
+    assert torch.equal(y, y2)
+    assert ((g.double() - (h.double() + d["dy"].double())).abs()
+            <= (h.abs() + d["dy"].abs()).double() * 2.0 ** -8).all()
+    cache = TF.mask_apply(d["weight"], d["mask"], BF16).requires_grad_()
+    w = d["weight"].clone().requires_grad_()
+    y = TF.masked_linear_act(d["x"], w, d["mask"], cache=cache)
+    a, b = torch.autograd.grad(y, (w, cache), d["dy"], allow_unused=True)
+    assert a is not None and b is None
+    big = quantize_act8(torch.cat((d["x"], d["x"]), 1).reshape(60, 48))
+    part = Act8(big.codes[::2], big.scales[::2])
+    whole = quantize_act8(d["x"])
+    gs = []
+    for k in (part, whole):
+        y = TF.masked_linear_act(d["x"], w, d["mask"], cache=cache,
+                                 keep="e4m3", kept=k)
+        gs.append(torch.autograd.grad(y, w, d["dy"])[0])
+    assert torch.equal(*gs)
+    check(dict(d, weight=d["weight"].half()), BF16, "gelu", "e4m3")
+
+
+@pytest.mark.parametrize("dev", DEVICES)
 def test_cast_inputs_and_cache(dev):
     """A float32 stream into a bfloat16 layer, as under autocast; a cache in
     place of weight and mask."""

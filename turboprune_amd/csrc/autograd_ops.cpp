@@ -3,6 +3,7 @@
 // one call from Python and none from the backward pass (in Python the same
 // steps take 40 us of a small layer's 80). CPU tensors never come here: their
 // plain form is ops/norm_act.py and ops/functional.py.
+#include <c10/core/DeviceGuard.h>
 #include <torch/extension.h>
 
 namespace turboprune {
@@ -206,6 +207,7 @@ at::Tensor gelu_keep8(const at::Tensor& x) {
   check_float("gelu", "x", x);
   TORCH_CHECK_VALUE(x.dim() >= 1,
                     "gelu(keep=...): a tensor of at least one dimension");
+  c10::DeviceGuard guard(x.device());
   return GeluKeep8::apply(x);
 }
 
@@ -214,6 +216,7 @@ std::tuple<at::Tensor, at::Tensor, OptTensor, OptTensor> add_rms_norm(
     double eps, const c10::optional<std::string>& keep_arg,
     c10::optional<at::ScalarType> out_dtype) {
   const char* op = "add_rms_norm";
+  c10::DeviceGuard guard(x.device());
   bool keep = keeps(keep_arg);
   check_float(op, "x", x);
   check_float(op, "weight", weight);
@@ -257,6 +260,7 @@ at::Tensor masked_linear_act(
     const c10::optional<std::string>& keep_arg, const OptTensor& codes,
     const OptTensor& scales) {
   const char* op = "masked_linear_act";
+  c10::DeviceGuard guard(x_in.device());
   bool keep = keeps(keep_arg);
   TORCH_CHECK_VALUE(!act_arg || *act_arg == "gelu", "act='",
                     act_arg ? *act_arg : "", "': None or 'gelu'");
@@ -314,11 +318,11 @@ at::Tensor masked_linear_act(
   }
   at::Tensor w;
   if (cache) {
-    w = *cache;
+    w = cache->detach();
   } else {
     at::NoGradGuard no_grad;
     if (!mask)
-      w = weight.to(ct);
+      w = weight.detach().to(ct);
     else if (weight.scalar_type() == at::kFloat && ct == at::kBFloat16)
       w = mask_apply(weight, *mask, ct);
     else

@@ -44,7 +44,7 @@ def check_float(name: str, t: torch.Tensor) -> None:
 class Act8(NamedTuple):
     """A tensor in the 8-bit format: ``codes`` (float8_e4m3fn, the tensor's
     shape) and ``scales`` (float8_e8m0fnu, one for every 32 values of the
-    last dimension)."""
+    last dimension, from 2^-126 to 2^126)."""
 
     codes: torch.Tensor
     scales: torch.Tensor

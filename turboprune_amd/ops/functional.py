@@ -281,7 +281,7 @@ def masked_linear_act(x: torch.Tensor, weight: torch.Tensor,
         raise TypeError(f"masked_linear_act: mask is {mask.dtype}: float32 "
                         "expected")
     if cache is not None:
-        w = cache
+        w = cache.detach()
     else:
         ct = compute_dtype or (weight.dtype if weight.dtype != torch.float32
                                else x.dtype)
