@@ -57,6 +57,17 @@ def test_kept_layer_norm_model_is_the_plain_one(dev):
 
 
 @pytest.mark.parametrize("dev", DEVICES)
+def test_fused_products_alone(dev):
+    plain, fused = vit(dev), vit(dev, fused=True)
+    fused.load_state_dict(plain.state_dict())
+    (a, ga), (b, gb) = step(plain, dev), step(fused, dev)
+    tol = 1e-5 if dev == "cpu" else 2.0 ** -5
+    assert abs(a - b) < tol
+    for n in ga:
+        assert (ga[n] - gb[n]).norm() < tol * ga[n].norm() + 1e-9, n
+
+
+@pytest.mark.parametrize("dev", DEVICES)
 def test_rms_model_against_its_formulas(dev):
     """Without keeping: the same model from elementary operations in 64
     bits."""
@@ -126,7 +137,7 @@ def test_config():
     m = build_model(cfg, num_classes=10).model
     assert m.blocks[0].keep == "e4m3"
     assert type(m.blocks[0].norm2).__name__ == "FusedRMSNorm"
-    for over in ("+model_params.norm=batch",
+    for over in ("+model_params.norm=batch", "+model_params.fused_products=2",
                  "+model_params.keep_activations=int8"):
         with pytest.raises(ConfigError):
             validate_config(compose("imagenet_deit_lrr", [over]))

@@ -81,6 +81,8 @@ def validate_config(cfg: Any) -> None:
     _choice(cfg, "model_params", "norm", NORMS, errors, required=False)
     _choice(cfg, "model_params", "keep_activations", KEPT_FORMATS, errors,
             required=False)
+    _choice(cfg, "model_params", "fused_products", (True, False), errors,
+            required=False)
 
     # pruning_params
     method = _choice(cfg, "pruning_params", "prune_method", PRUNE_METHODS, errors)

@@ -294,7 +294,10 @@ TP_DEVICE void add8(const T* p, int n, float (&v)[8]) {
 
 // v: the sums of 8 neighbouring columns of one row; n of them exist (<= 0:
 // none; FULL: all). The lanes l, l^16, l^32 and l^48 hold one 32-column block.
-template <typename T, int ACT, bool FULL>
+// PLAIN: no residual, no mask, 16-bit output, known beforehand (choosing here
+// costs the registers' moves where the choices meet again, a tenth of the
+// epilogue).
+template <typename T, int ACT, bool FULL, bool PLAIN>
 TP_DEVICE void epilogue8(const Epi& e, int64_t at, int64_t blk, int n,
                          bool first, float (&v)[8]) {
   if constexpr (ACT == kGelu8) {
@@ -310,6 +313,10 @@ TP_DEVICE void epilogue8(const Epi& e, int64_t at, int64_t blk, int n,
   if constexpr (ACT != kNoAct)
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = gelu_short(v[i]);
+  if constexpr (PLAIN) {
+    put8<FULL>((T*)e.out + at, n, v);
+    return;
+  }
   if (e.res) {
     if (e.res_f32)
       add8<FULL>((const float*)e.res + at, n, v);
@@ -330,7 +337,7 @@ TP_DEVICE void epilogue8(const Epi& e, int64_t at, int64_t blk, int n,
 }
 
 template <typename T, int BQ, int BP, int BK, int WQ, int WP, int QF, int PF,
-          int STAGES, int MINW, int ACT>
+          int STAGES, int MINW, int ACT, bool PLAIN>
 __global__ __launch_bounds__(WQ * WP * 64, MINW) void mm_kernel(Mm a) {
   constexpr int NW = WQ * WP;
   constexpr bool QTR = QF != kRowK, PTR = PF != kRowK;
@@ -451,7 +458,7 @@ __global__ __launch_bounds__(WQ * WP * 64, MINW) void mm_kernel(Mm a) {
           v[k] = __uint_as_float(s[0]);
           v[4 + k] = __uint_as_float(s[1]);
         }
-        epilogue8<T, ACT, FULL>(a.e, at + i * 16, blk + i / 2,
+        epilogue8<T, ACT, FULL, PLAIN>(a.e, at + i * 16, blk + i / 2,
                                 row < a.M ? a.N - c0 - i * 16 : 0, g == 0, v);
       }
     }
@@ -588,7 +595,7 @@ __global__ __launch_bounds__(512) void rows_kernel(Mm a) {
     v[4 + k] = __uint_as_float(t[1]);
   }
   int c0 = n0 + (g & 1) * 16 + (g >> 1) * 8;
-  epilogue8<T, ACT, false>(
+  epilogue8<T, ACT, false, false>(
       a.e, (int64_t)row * a.N + c0,
       (int64_t)row * ((a.N + 31) / 32) + blockIdx.x,
       row < a.M ? a.N - c0 : 0, g == 0, v);
@@ -790,12 +797,20 @@ int64_t row_bytes(const at::Tensor& t) {
 template <typename T, int BQ, int BP, int BK, int WQ, int WP, int QF, int PF,
           int ST, int MINW, int ACT = kNoAct>
 void launch_mm(Mm a, int slabs = 1) {
+  // across the sum (weight gradients) the output is masked or in slabs
+  constexpr bool kRows = PF == kRowK;
+  bool plain = kRows && !a.e.res && !a.e.mask && !a.e.out_f32;
   a.tiles_n = (a.N + BP - 1) / BP;
   a.tiles = (a.M + BQ - 1) / BQ * a.tiles_n;
   int kt = (a.K + BK - 1) / BK;
   a.kper = (kt + slabs - 1) / slabs;
-  mm_kernel<T, BQ, BP, BK, WQ, WP, QF, PF, ST, MINW, ACT>
-      <<<dim3(a.tiles, slabs), WQ * WP * 64, 0, current()>>>(a);
+  dim3 grid(a.tiles, slabs);
+  if (kRows && plain)
+    mm_kernel<T, BQ, BP, BK, WQ, WP, QF, PF, ST, MINW, ACT, kRows>
+        <<<grid, WQ * WP * 64, 0, current()>>>(a);
+  else
+    mm_kernel<T, BQ, BP, BK, WQ, WP, QF, PF, ST, MINW, ACT, false>
+        <<<grid, WQ * WP * 64, 0, current()>>>(a);
   C10_HIP_KERNEL_LAUNCH_CHECK();
 }
 

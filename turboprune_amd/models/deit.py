@@ -12,11 +12,12 @@ latent-broken. This is a working native implementation:
 - attention itself uses torch SDPA on ROCm; the masked qkv/proj/mlp
   projections are the MFMA masked-GEMM hot path.
 
-Two options beyond the reference, off by default, make a block run on the
-fused operators (``Block._fused``): ``norm="rms"`` takes root-mean-square
+Options beyond the reference, off by default, make a block run on the fused
+operators (``Block._fused``), with bias, GELU and residual in the products'
+epilogues: ``fused=True`` is that alone, ``norm="rms"`` takes root-mean-square
 norms that add the residual on the way, ``keep="e4m3"`` holds what the linear
-layers and the MLP's GELU need for the backward pass in 8 bits. Either way the
-bias, GELU and residual are in the products' epilogues.
+layers and the MLP's GELU need for the backward pass in 8 bits. They compute in
+16 bits on a GPU: under autocast or with the layers' caches enabled.
 """
 
 from __future__ import annotations
@@ -133,17 +134,19 @@ class Mlp(nn.Module):
 class Block(nn.Module):
     def __init__(self, dim, num_heads, mlp_ratio=4.0, qkv_bias=True,
                  drop=0.0, attn_drop=0.0, norm_layer=nn.LayerNorm,
-                 keep=None):
+                 keep=None, fused=False):
         super().__init__()
         check_keep(keep)
         self.keep = keep
+        self.fused = fused
         self.norm1 = norm_layer(dim)
         self.attn = Attention(dim, num_heads, qkv_bias, attn_drop, drop)
         self.norm2 = norm_layer(dim)
         self.mlp = Mlp(dim, int(dim * mlp_ratio), drop)
 
     def forward(self, x):
-        if self.keep is not None or isinstance(self.norm1, FusedRMSNorm):
+        if self.fused or self.keep is not None \
+                or isinstance(self.norm1, FusedRMSNorm):
             return self._fused(x)
         x = x + self.attn(self.norm1(x))
         x = x + self.mlp(self.norm2(x))
@@ -166,7 +169,7 @@ class VisionTransformer(nn.Module):
                  num_classes=1000, embed_dim=768, depth=12, num_heads=12,
                  mlp_ratio=4.0, qkv_bias=True, drop_rate=0.0,
                  attn_drop_rate=0.0, norm_layer=None, norm="layer",
-                 keep=None):
+                 keep=None, fused=False):
         super().__init__()
         if norm not in NORMS:
             raise ValueError(f"norm={norm!r}: one of {tuple(NORMS)}")
@@ -181,7 +184,7 @@ class VisionTransformer(nn.Module):
         self.pos_drop = nn.Dropout(drop_rate)
         self.blocks = nn.ModuleList([
             Block(embed_dim, num_heads, mlp_ratio, qkv_bias, drop_rate,
-                  attn_drop_rate, norm_layer, keep)
+                  attn_drop_rate, norm_layer, keep, fused)
             for _ in range(depth)])
         self.norm = norm_layer(embed_dim)
         self.head = Conv1dMask(embed_dim, num_classes, bias=True) \

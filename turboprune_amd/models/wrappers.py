@@ -148,8 +148,9 @@ def build_model(cfg: Any, num_classes: Optional[int] = None) -> PruneModel:
     """Construct the masked model named by ``cfg.model_params.model_name``
     (resnet*/vgg*/local_deit_*), with CIFAR stem surgery for CIFAR
     datasets (reference: custom_models.py:169-245, fixed DeiT path).
-    ``model_params.norm`` and ``model_params.keep_activations`` choose the
-    local_deit_* models' norm and what they keep for the backward pass."""
+    ``model_params.norm``, ``model_params.keep_activations`` and
+    ``model_params.fused_products`` choose the local_deit_* models' norm, what
+    they keep for the backward pass, and the products with an epilogue."""
     name = cfg.model_params.model_name
     dataset = cfg.dataset_params.dataset_name
     if num_classes is None:
@@ -172,7 +173,8 @@ def build_model(cfg: Any, num_classes: Optional[int] = None) -> PruneModel:
     kwargs = {"num_classes": num_classes}
     if name.startswith(("resnet", "vgg")):
         kwargs["cifar_stem"] = dataset in ("CIFAR10", "CIFAR100")
-    for key, arg in (("norm", "norm"), ("keep_activations", "keep")):
+    for key, arg in (("norm", "norm"), ("keep_activations", "keep"),
+                     ("fused_products", "fused")):
         value = cfg.select(f"model_params.{key}", None)
         if value is not None:
             if not name.startswith("local_deit"):
