@@ -233,7 +233,7 @@ template <typename T, int BQ, int BK, int THREADS>
 TP_DEVICE void keep_tile(TP_LDS const char* t, const Mm& a, int m0, int kt) {
   constexpr int C = BK / 8;
   static_assert(BQ * C % THREADS == 0, "whole rounds");
-#pragma unroll
+#pragma unroll 1   // registers are short beside the sums
   for (int i = 0; i < BQ * C / THREADS; ++i) {
     int at = i * THREADS + threadIdx.x, r = at / C, c = at % C;
     u32x4 d = *reinterpret_cast<TP_LDS const u32x4*>(
@@ -269,6 +269,13 @@ struct LanesMax {   // over lanes l, l^16, l^32, l^48
     return fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
   }
 };
+
+// When a k-tile's successor is fetched: behind the reads of the first
+// fragments (the waves' first products then do not wait behind address
+// arithmetic: 131 -> 120 us for 50432x1536x384 with GELU and codes), behind
+// those of all, or between the two halves of the products. Which is best goes
+// by the registers that are left: all fragments of 16 waves at once spill.
+enum { kAfterFirst = 0, kAfterReads = 1, kBetween = 2 };
 
 // What follows the sum: nothing but the residual, GELU with z kept in 16 bits
 // (or not at all), GELU with z kept in 8.
@@ -337,7 +344,7 @@ TP_DEVICE void epilogue8(const Epi& e, int64_t at, int64_t blk, int n,
 }
 
 template <typename T, int BQ, int BP, int BK, int WQ, int WP, int QF, int PF,
-          int STAGES, int MINW, int ACT, bool PLAIN>
+          int STAGES, int MINW, int WHEN, int ACT, bool PLAIN>
 __global__ __launch_bounds__(WQ * WP * 64, MINW) void mm_kernel(Mm a) {
   constexpr int NW = WQ * WP;
   constexpr bool QTR = QF != kRowK, PTR = PF != kRowK;
@@ -407,30 +414,53 @@ __global__ __launch_bounds__(WQ * WP * 64, MINW) void mm_kernel(Mm a) {
       wait_and_meet<(STAGES - 2) * LOADS>();
     else
       wait_and_meet<0>();
-    // every wave has read tile kt - 1, whose place tile kt + STAGES - 1 takes
-    if (kt + STAGES - 1 < kt1) fetch(kt + STAGES - 1);
-    if constexpr (PF == kCodes) {
-      if (kt + 1 < kt1) ct.store(place(kt + 1) + QB);
-      if (kt + 2 < kt1) ct.load(a, n0, kt + 2);
-    }
+    // Every wave has read tile kt - 1, whose place tile kt + STAGES - 1 takes.
     TP_LDS const char* b = place(kt);
-    if constexpr (QF == kRowK && PF == kRowK)
-      if (a.qcodes && kt % a.tiles_n == wg % a.tiles_n)
-        keep_tile<T, BQ, BK, NW * 64>(b, a, m0, kt);
-#pragma unroll
-    for (int ks = 0; ks < BK / 32; ++ks) {
-      s16x8 fq[MI], fp[NI];
+    auto more = [&]() {
+      if (kt + STAGES - 1 < kt1) fetch(kt + STAGES - 1);
+      if constexpr (PF == kCodes) {
+        if (kt + 1 < kt1) ct.store(place(kt + 1) + QB);
+        if (kt + 2 < kt1) ct.load(a, n0, kt + 2);
+      }
+    };
+    constexpr int KS = BK / 32;
+    s16x8 fq[KS][MI], fp[KS][NI];
+    auto read = [&](int ks) {
 #pragma unroll
       for (int i = 0; i < MI; ++i)
-        fq[i] = frag<BQ, BK, QTR>(b, wq + i * 16, ks, lane);
+        fq[ks][i] = frag<BQ, BK, QTR>(b, wq + i * 16, ks, lane);
 #pragma unroll
       for (int i = 0; i < NI; ++i)
-        fp[i] = frag<BP, BK, PTR>(b + QB, wp + i * 16, ks, lane);
+        fp[ks][i] = frag<BP, BK, PTR>(b + QB, wp + i * 16, ks, lane);
+    };
+    auto multiply = [&](int ks) {
 #pragma unroll
       for (int i = 0; i < NI; ++i)
 #pragma unroll
         for (int j = 0; j < MI; ++j)
-          acc[i][j] = mma<T>(fp[i], fq[j], acc[i][j]);
+          acc[i][j] = mma<T>(fp[ks][i], fq[ks][j], acc[i][j]);
+    };
+    read(0);
+    if constexpr (WHEN == kAfterFirst) {
+      more();
+      multiply(0);
+#pragma unroll
+      for (int ks = 1; ks < KS; ++ks) {
+        read(ks);
+        multiply(ks);
+      }
+      // last, when no fragment is alive
+      if constexpr (QF == kRowK && PF == kRowK)
+        if (a.qcodes && kt % a.tiles_n == wg % a.tiles_n)
+          keep_tile<T, BQ, BK, NW * 64>(b, a, m0, kt);
+    } else {
+#pragma unroll
+      for (int ks = 1; ks < KS; ++ks) read(ks);
+      if constexpr (WHEN == kAfterReads) more();
+      multiply(0);
+      if constexpr (WHEN == kBetween) more();
+#pragma unroll
+      for (int ks = 1; ks < KS; ++ks) multiply(ks);
     }
   }
 
@@ -795,7 +825,7 @@ int64_t row_bytes(const at::Tensor& t) {
 }
 
 template <typename T, int BQ, int BP, int BK, int WQ, int WP, int QF, int PF,
-          int ST, int MINW, int ACT = kNoAct>
+          int ST, int MINW, int WHEN, int ACT = kNoAct>
 void launch_mm(Mm a, int slabs = 1) {
   // across the sum (weight gradients) the output is masked or in slabs
   constexpr bool kRows = PF == kRowK;
@@ -806,10 +836,12 @@ void launch_mm(Mm a, int slabs = 1) {
   a.kper = (kt + slabs - 1) / slabs;
   dim3 grid(a.tiles, slabs);
   if (kRows && plain)
-    mm_kernel<T, BQ, BP, BK, WQ, WP, QF, PF, ST, MINW, ACT, kRows>
+    mm_kernel<T, BQ, BP, BK, WQ, WP, QF, PF, ST, MINW, WHEN, ACT,
+              kRows>
         <<<grid, WQ * WP * 64, 0, current()>>>(a);
   else
-    mm_kernel<T, BQ, BP, BK, WQ, WP, QF, PF, ST, MINW, ACT, false>
+    mm_kernel<T, BQ, BP, BK, WQ, WP, QF, PF, ST, MINW, WHEN, ACT,
+              false>
         <<<grid, WQ * WP * 64, 0, current()>>>(a);
   C10_HIP_KERNEL_LAUNCH_CHECK();
 }
@@ -850,20 +882,22 @@ void run_few(const Mm& a) {
 template <typename T, int ACT>
 void run_rows(const Mm& a) {
   if (tiles_of(a, 64, 64) <= 600)
-    return launch_mm<T, 64, 64, 64, 2, 2, kRowK, kRowK, 2, 1, ACT>(a);
+    return launch_mm<T, 64, 64, 64, 2, 2, kRowK, kRowK, 2, 1, kAfterFirst, ACT>(
+        a);
   int64_t t = tiles_of(a, 256, 256);
   bool filled = (a.N + 255) / 256 * 256 <= a.N + a.N / 5;
   if (filled && t >= 200 && (a.K >= 512 || t >= 768))
-    return launch_mm<T, 256, 256, 64, 4, 4, kRowK, kRowK, 2, 4, ACT>(a);
-  launch_mm<T, 128, 128, 64, 2, 4, kRowK, kRowK, 2, 2, ACT>(a);
+    return launch_mm<T, 256, 256, 64, 4, 4, kRowK, kRowK, 2, 4, kAfterFirst,
+                     ACT>(a);
+  launch_mm<T, 128, 128, 64, 2, 4, kRowK, kRowK, 2, 2, kAfterFirst, ACT>(a);
 }
 
 // Both across the sum (weight gradients), in slabs of it: as many as fill the
-// chip, none shorter than four k-tiles. 4096x1024 over 25216 rows takes 204 us
-// in 256 x 256 tiles and 235 in 128 x 128; 1536x384 over 50432 rows 87 us in
-// 128 x 128 and 97 in 256 x 256, whose third column tile is half empty.
+// chip, none shorter than four k-tiles. 4096x1024 over 25216 rows takes 197 us
+// in 256 x 256 tiles and 235 in 128 x 128; 1536x384 over 50432 rows 88 us in
+// 128 x 128 and 95 in 256 x 256, whose third column tile is half empty.
 // Codes go through registers, which 16 waves leave too few of: 8 waves there
-// (253 us against 285; 128 x 128 336).
+// (200 us against 285; 128 x 128 266).
 struct Split {
   int tile, slabs;
 };
@@ -883,13 +917,16 @@ template <typename T, int PF>
 void run_cols(const Mm& a, Split s) {
   if (s.tile == 256) {
     if constexpr (PF == kCodes)
-      return launch_mm<T, 256, 256, 64, 2, 4, kColK, PF, 2, 2>(a, s.slabs);
+      return launch_mm<T, 256, 256, 64, 2, 4, kColK, PF, 2, 2, kBetween>(
+          a, s.slabs);
     else
-      return launch_mm<T, 256, 256, 64, 4, 4, kColK, PF, 2, 4>(a, s.slabs);
+      return launch_mm<T, 256, 256, 64, 4, 4, kColK, PF, 2, 4, kAfterFirst>(
+          a, s.slabs);
   }
   if (s.tile == 128)
-    return launch_mm<T, 128, 128, 64, 2, 4, kColK, PF, 2, 2>(a, s.slabs);
-  launch_mm<T, 64, 64, 64, 2, 2, kColK, PF, 2, 1>(a, s.slabs);
+    return launch_mm<T, 128, 128, 64, 2, 4, kColK, PF, 2, 2, kAfterReads>(
+        a, s.slabs);
+  launch_mm<T, 64, 64, 64, 2, 2, kColK, PF, 2, 1, kAfterReads>(a, s.slabs);
 }
 
 void check_size(int64_t M, int64_t N, int64_t K) {
@@ -1113,7 +1150,8 @@ linear_act_bwd(const at::Tensor& dy_in, const c10::optional<at::Tensor>& z,
       a.ldp = row_bytes(wl);
       a.np = (int)wl.size(1);
       by16(st, [&](auto t) {
-        launch_mm<decltype(t), 64, 64, 64, 2, 2, kRowK, kColK, 2, 1>(a);
+        launch_mm<decltype(t), 64, 64, 64, 2, 2, kRowK, kColK, 2, 1,
+                  kAfterFirst>(a);
       });
     }
   }
