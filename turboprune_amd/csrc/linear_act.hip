@@ -233,21 +233,30 @@ template <typename T, int BQ, int BK, int THREADS>
 TP_DEVICE void keep_tile(TP_LDS const char* t, const Mm& a, int m0, int kt) {
   constexpr int C = BK / 8;
   static_assert(BQ * C % THREADS == 0, "whole rounds");
-#pragma unroll 1   // registers are short beside the sums
-  for (int i = 0; i < BQ * C / THREADS; ++i) {
-    int at = i * THREADS + threadIdx.x, r = at / C, c = at % C;
-    u32x4 d = *reinterpret_cast<TP_LDS const u32x4*>(
-        t + r * (BK * 2) + (c ^ Tile<BQ, BK, false>::swap(r)) * 16);
-    float v[8];
-    unpack8<T>(d, v);
-    int e, col = kt * BK + c * 8;
-    uint2 q = encode8(v, e, QuadMax());
-    int64_t row = m0 + r;
-    int n = row < a.M ? a.K - col : 0;
-    if (n <= 0) continue;
-    store_codes(a.qcodes + row * a.K + col, n, q);
-    if ((c & 3) == 0)
-      a.qscale[row * ((a.K + 31) / 32) + col / 32] = (uint8_t)(e + 127);
+  // all rounds at once where registers allow, one by one beside 16 waves' sums
+  constexpr int R = BQ * C / THREADS, U = THREADS == 1024 ? 1 : R;
+#pragma unroll 1
+  for (int i0 = 0; i0 < R; i0 += U) {
+    float v[U][8];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      int at = (i0 + u) * THREADS + threadIdx.x, r = at / C, c = at % C;
+      unpack8<T>(*reinterpret_cast<TP_LDS const u32x4*>(
+                     t + r * (BK * 2) + (c ^ Tile<BQ, BK, false>::swap(r)) * 16),
+                 v[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      int at = (i0 + u) * THREADS + threadIdx.x, r = at / C, c = at % C;
+      int e, col = kt * BK + c * 8;
+      uint2 q = encode8(v[u], e, QuadMax());
+      int64_t row = m0 + r;
+      int n = row < a.M ? a.K - col : 0;
+      if (n <= 0) continue;
+      store_codes(a.qcodes + row * a.K + col, n, q);
+      if ((c & 3) == 0)
+        a.qscale[row * ((a.K + 31) / 32) + col / 32] = (uint8_t)(e + 127);
+    }
   }
 }
 
