@@ -536,6 +536,17 @@ def test_few_rows(dev, t, M, K, N):
         assert ((y.double() - want).abs() <= tol).all()
 
 
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("t", [BF16, FP16])
+@pytest.mark.parametrize("M,K,N", [
+    (100, 768, 384), (197, 384, 1536), (200, 97, 1100), (256, 300, 2048),
+    (128, 64, 4096), (300, 131, 1000), (4096, 34, 31), (4097, 34, 31),
+    (16, 72, 9000), (32, 71, 9000), (40, 72, 9000)])
+def test_rows_in_groups(dev, t, M, K, N):
+    """Few outputs in all, whatever their rows and columns."""
+    test_few_rows(dev, t, M, K, N)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("t", [BF16, FP16])
 @pytest.mark.parametrize("M,K,N", [
@@ -621,8 +632,10 @@ def test_rows_past_32_bit_offsets():
     x[-100:] = d["x"]
     y = TF.masked_linear_act(x, d["weight"], d["mask"], d["bias"],
                              act="gelu", compute_dtype=BF16)
-    ref = TF.masked_linear_act(d["x"], d["weight"], d["mask"], d["bias"],
-                               act="gelu", compute_dtype=BF16)
+    # a call with gradients: 100 rows alone would be added in another order
+    ref = TF.masked_linear_act(d["x"], d["weight"].clone().requires_grad_(),
+                               d["mask"], d["bias"], act="gelu",
+                               compute_dtype=BF16).detach()
     assert torch.equal(y[-100:], ref)
     assert torch.equal(y[:1].expand(1000, N), y[:1000])
     del y

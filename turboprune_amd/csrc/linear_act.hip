@@ -508,11 +508,14 @@ __global__ __launch_bounds__(WQ * WP * 64, MINW) void mm_kernel(Mm a) {
     finish(std::false_type());
 }
 
-// Few rows (single tokens, a classifier's batch): the weight is read once and
-// nothing is used twice, so there are no tiles to stage. A block takes 32
-// columns; its 8 waves take 32 values of k each in turn, straight from global
-// memory into fragments (rows at any address), and their sums meet in LDS, wave
-// j finishing 16 rows. The staged kernel would give 29x2875x768 to 12 CUs.
+// Few rows (single tokens, one image, a classifier's batch): nothing is used
+// often enough for tiles to pay, and the staged kernel would give 29x2875x768
+// to 12 CUs, each waiting for 45 loads in turn. A block takes 32 columns and
+// MI x 16 rows; its 8 waves take 32 values of k each in turn, straight from
+// global memory into fragments (rows at any address), and their sums meet in
+// LDS, wave j finishing 16 rows. Bound by the latency of the few steps that
+// each wave makes (1x384x1000 and 1x768x768 3.7 and 4.3 us), then by what a
+// block reads: 1x4096x4096 13 us, 2.6 TB/s, weights from memory.
 //
 // 8 values of a row from p on. Where rows have an odd length they start between
 // two dwords every other time, and a 16-byte load there is taken apart by the
@@ -554,13 +557,13 @@ __global__ __launch_bounds__(512) void rows_kernel(Mm a) {
   __shared__ f32x4 part[NW][2 * MI][64];
   int lane = threadIdx.x & 63, g = lane >> 4;
   int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-  int n0 = blockIdx.x * 32;
+  int n0 = blockIdx.x * 32, m0 = blockIdx.y * (MI * 16);
   // rows behind the last are the last one again: what they give is not stored
   const T* q[MI];
   const T* p[2];
 #pragma unroll
   for (int j = 0; j < MI; ++j)
-    q[j] = (const T*)(a.q + min(j * 16 + (lane & 15), a.M - 1) * a.ldq);
+    q[j] = (const T*)(a.q + min(m0 + j * 16 + (lane & 15), a.M - 1) * a.ldq);
 #pragma unroll
   for (int i = 0; i < 2; ++i)
     p[i] = (const T*)(a.p + min(n0 + i * 16 + (lane & 15), a.N - 1) * a.ldp);
@@ -610,7 +613,7 @@ __global__ __launch_bounds__(512) void rows_kernel(Mm a) {
     for (int j = 0; j < MI; ++j) part[wave][i * MI + j][lane] = acc[i][j];
   __syncthreads();
   if (wave >= MI) return;
-  int j = wave, row = j * 16 + (lane & 15);
+  int j = wave, row = m0 + j * 16 + (lane & 15);
   f32x4 s[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
@@ -859,24 +862,30 @@ int64_t tiles_of(const Mm& a, int q, int p) {
   return (int64_t)((a.M + q - 1) / q) * ((a.N + p - 1) / p);
 }
 
-// Both operands along the sum. 256 x 256 by 16 waves moves the fewest bytes
-// into LDS per product, but it needs about a CU each to pay, little of the last
-// column tile empty, and it ends with an epilogue that no other block's product
-// hides: 50432x1536x384 in 92 us against 105 with 128 x 128, 25216x1024x4096
-// in 214 against 258; but 50432x384x1536 with a 32-bit residual (a third of
-// the columns empty) in 138 against 116, 12608x1536x384 (300 tiles, two rounds
-// for little more than one) in 32 against 26. Short products end soonest in
-// many small tiles: 1576x768x768 10.2 us in 64 x 64, 12.0 in 128 x 128;
-// 3152x1536x384 (1200 small tiles) 13.8 against 12.9.
+// Groups of 16 rows that a block of rows_kernel takes, 0: the tiles. Such
+// blocks hold little and read much, so they win while the chip has a CU for
+// each, and the smallest that still have one win most (fp16, us, with 1, 2
+// and 4 groups to a block, and the staged kernel in 64 x 64): 64x4096x1024
+// 13.4, 16.8, 23.7, 32.6; 197x768x768 6.7, 5.6, 6.9, 7.3; 128x4096x4096 (128
+// column blocks, so 4 groups) 47, 32, 25, 34. Past that many blocks the tiles
+// win, 197x1024x4096 in 11.6 against 14.7, but for a weight that is read once
+// all the same: 16x1024x16384 8.2 against 11.5, 32 rows 10.0 against 11.6, 64
+// rows 15.2 against 11.6.
+int row_groups(int64_t M, int64_t N) {
+  int64_t cols = (N + 31) / 32;
+  for (int g = 1; g <= 4; g *= 2)
+    if ((M + g * 16 - 1) / (g * 16) * cols <= 256) return g;
+  return M <= 16 ? 1 : M <= 32 ? 2 : 0;
+}
 template <typename T, int ACT>
-void run_few(const Mm& a) {
-  unsigned grid = (unsigned)((a.N + 31) / 32);
+void run_few(const Mm& a, int groups) {
+  dim3 grid((a.N + 31) / 32, (a.M + groups * 16 - 1) / (groups * 16));
   auto run = [&](auto odd) {
     constexpr bool ODD = decltype(odd)::value;
     auto s = current();
-    if (a.M <= 16)
+    if (groups == 1)
       rows_kernel<T, 1, ACT, ODD><<<grid, 512, 0, s>>>(a);
-    else if (a.M <= 32)
+    else if (groups == 2)
       rows_kernel<T, 2, ACT, ODD><<<grid, 512, 0, s>>>(a);
     else
       rows_kernel<T, 4, ACT, ODD><<<grid, 512, 0, s>>>(a);
@@ -888,6 +897,15 @@ void run_few(const Mm& a) {
     run(std::false_type());
 }
 
+// Both operands along the sum. 256 x 256 by 16 waves moves the fewest bytes
+// into LDS per product, but it needs about a CU each to pay, little of the last
+// column tile empty, and it ends with an epilogue that no other block's product
+// hides: 50432x1536x384 in 92 us against 105 with 128 x 128, 25216x1024x4096
+// in 214 against 258; but 50432x384x1536 with a 32-bit residual (a third of
+// the columns empty) in 138 against 116, 12608x1536x384 (300 tiles, two rounds
+// for little more than one) in 32 against 26. Short products end soonest in
+// many small tiles: 1576x768x768 10.2 us in 64 x 64, 12.0 in 128 x 128;
+// 3152x1536x384 (1200 small tiles) 13.8 against 12.9.
 template <typename T, int ACT>
 void run_rows(const Mm& a) {
   if (tiles_of(a, 64, 64) <= 600)
@@ -992,7 +1010,7 @@ linear_act_fwd(const at::Tensor& x, const at::Tensor& w,
   // few rows without a backward pass to come (in training every sum is the
   // tiles', so that it does not go by what is kept); they need neither
   // alignment nor padding
-  bool few = M <= 64 && keep == 0 && !keep_x;
+  int few = keep == 0 && !keep_x ? row_groups(M, N) : 0;
   auto in_rows = [](const at::Tensor& t) {
     return t.size(1) <= 1 || t.stride(1) == 1 ? t : t.contiguous();
   };
@@ -1021,7 +1039,7 @@ linear_act_fwd(const at::Tensor& x, const at::Tensor& w,
   by16(st, [&](auto t) {
     using T = decltype(t);
     if (few)
-      act ? run_few<T, kGelu>(a) : run_few<T, kNoAct>(a);
+      act ? run_few<T, kGelu>(a, few) : run_few<T, kNoAct>(a, few);
     else if (!act)
       run_rows<T, kNoAct>(a);
     else if (zs)
