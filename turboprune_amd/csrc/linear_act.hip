@@ -22,6 +22,7 @@ using namespace act8;
 
 std::pair<at::Tensor, at::Tensor> act8_empty(at::IntArrayRef,
                                              const at::TensorOptions&);
+std::tuple<at::Tensor, at::Tensor> act8_quantize(const at::Tensor&);
 
 namespace {
 
@@ -67,7 +68,6 @@ struct Mm {
   int64_t ldq, ldp;      // row distance in bytes
   int nq, np;            // rows (kRowK) or columns (kColK) that can be read
   const uint8_t* pscale; // kCodes: a scale for every 32 codes of a row
-  uint8_t *qcodes, *qscale;   // kRowK: Q in 8 bits, to be written, or null
   int M, N, K;           // rows and columns of C, length of the sum
   int tiles_n, tiles;    // tile grid
   int ksplit, kper;      // k-tiles of one slab; slab s writes out + s M N
@@ -224,41 +224,6 @@ struct CodeTile {
     }
   }
 };
-
-// Q's values of one k-tile, from LDS, in 8 bits. The column tiles of a row of
-// tiles take the k-tiles in turn, so that each of them does its share and the
-// input is read once for product and codes (a pass of its own over 50432 x
-// 1536 values takes 42 us).
-template <typename T, int BQ, int BK, int THREADS>
-TP_DEVICE void keep_tile(TP_LDS const char* t, const Mm& a, int m0, int kt) {
-  constexpr int C = BK / 8;
-  static_assert(BQ * C % THREADS == 0, "whole rounds");
-  // all rounds at once where registers allow, one by one beside 16 waves' sums
-  constexpr int R = BQ * C / THREADS, U = THREADS == 1024 ? 1 : R;
-#pragma unroll 1
-  for (int i0 = 0; i0 < R; i0 += U) {
-    float v[U][8];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      int at = (i0 + u) * THREADS + threadIdx.x, r = at / C, c = at % C;
-      unpack8<T>(*reinterpret_cast<TP_LDS const u32x4*>(
-                     t + r * (BK * 2) + (c ^ Tile<BQ, BK, false>::swap(r)) * 16),
-                 v[u]);
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      int at = (i0 + u) * THREADS + threadIdx.x, r = at / C, c = at % C;
-      int e, col = kt * BK + c * 8;
-      uint2 q = encode8(v[u], e, QuadMax());
-      int64_t row = m0 + r;
-      int n = row < a.M ? a.K - col : 0;
-      if (n <= 0) continue;
-      store_codes(a.qcodes + row * a.K + col, n, q);
-      if ((c & 3) == 0)
-        a.qscale[row * ((a.K + 31) / 32) + col / 32] = (uint8_t)(e + 127);
-    }
-  }
-}
 
 template <int N>
 TP_DEVICE void wait_and_meet() {
@@ -458,10 +423,6 @@ __global__ __launch_bounds__(WQ * WP * 64, MINW) void mm_kernel(Mm a) {
         read(ks);
         multiply(ks);
       }
-      // last, when no fragment is alive
-      if constexpr (QF == kRowK && PF == kRowK)
-        if (a.qcodes && kt % a.tiles_n == wg % a.tiles_n)
-          keep_tile<T, BQ, BK, NW * 64>(b, a, m0, kt);
     } else {
 #pragma unroll
       for (int ks = 1; ks < KS; ++ks) read(ks);
@@ -806,6 +767,13 @@ void by16(at::ScalarType t, F&& f) {
 
 hipStream_t current() { return at::hip::getCurrentHIPStream(); }
 
+// blocks of a launch, which may have fewer than 2^32 threads
+unsigned grid_of(int64_t blocks, int threads) {
+  TORCH_CHECK(blocks * threads < (int64_t(1) << 32),
+              "linear_act: a matrix too large for one launch");
+  return (unsigned)blocks;
+}
+
 constexpr int kMaxCols = 1 << 20;   // row offsets of a tile fit 31 bits
 
 // A 2-D matrix that the tiles can load: values of a row together, rows 16
@@ -824,8 +792,8 @@ at::Tensor loadable(const at::Tensor& t) {
   if (chunks)
     by16(t.scalar_type(), [&](auto z) {
       using T = decltype(z);
-      pad_kernel<T><<<(unsigned)((chunks + kBlock - 1) / kBlock), kBlock, 0,
-                      current()>>>(
+      pad_kernel<T><<<grid_of((chunks + kBlock - 1) / kBlock, kBlock), kBlock,
+                      0, current()>>>(
           (const T*)s.data_ptr(), (T*)out.data_ptr(), chunks, s.stride(0),
           (int)C, (int)(C8 / 8));
       C10_HIP_KERNEL_LAUNCH_CHECK();
@@ -843,7 +811,8 @@ void launch_mm(Mm a, int slabs = 1) {
   constexpr bool kRows = PF == kRowK;
   bool plain = kRows && !a.e.res && !a.e.mask && !a.e.out_f32;
   a.tiles_n = (a.N + BP - 1) / BP;
-  a.tiles = (a.M + BQ - 1) / BQ * a.tiles_n;
+  a.tiles = (int)grid_of((int64_t)((a.M + BQ - 1) / BQ) * a.tiles_n,
+                         WQ * WP * 64);
   int kt = (a.K + BK - 1) / BK;
   a.kper = (kt + slabs - 1) / slabs;
   dim3 grid(a.tiles, slabs);
@@ -897,26 +866,43 @@ void run_few(const Mm& a, int groups) {
     run(std::false_type());
 }
 
-// Both operands along the sum. 256 x 256 by 16 waves moves the fewest bytes
-// into LDS per product, but it needs about a CU each to pay, little of the last
-// column tile empty, and it ends with an epilogue that no other block's product
-// hides: 50432x1536x384 in 92 us against 105 with 128 x 128, 25216x1024x4096
-// in 214 against 258; but 50432x384x1536 with a 32-bit residual (a third of
-// the columns empty) in 138 against 116, 12608x1536x384 (300 tiles, two rounds
-// for little more than one) in 32 against 26. Short products end soonest in
-// many small tiles: 1576x768x768 10.2 us in 64 x 64, 12.0 in 128 x 128;
-// 3152x1536x384 (1200 small tiles) 13.8 against 12.9.
+// Both operands along the sum. Short products end soonest in many small tiles:
+// 1576x768x768 10.2 us in 64 x 64, 12.0 in 128 x 128; 3152x1536x384 (1200
+// small tiles) 13.8 against 12.9.
+//
+// Of the large tiles 256 x 256 by 16 waves moves the fewest bytes into LDS per
+// product, but a CU holds one, and one tile more than CUs doubles the time. Of
+// 160 x 128 by 4 waves and 128 x 128 by 8 a CU holds two, the epilogue of one
+// behind the product of the other. What decides is how often the CU that has
+// most has to begin anew; per value of the output the smaller ones take 1.2 and
+// 1.25 times as long, and an odd one, alone at the end, half as long again as
+// in company. Over 60 sizes (6304 to 50432 rows, N and K of 384 to 4096, with
+// and without a 32-bit residual) this finds the fastest within 1 % on average
+// and 14 % at most; 256 x 256 wherever it is well filled, else 128 x 128, is
+// 7 % and 47 % off. In us, 256 x 256, 160 x 128, 128 x 128:
+//   50432x1536x384, GELU, codes   118  135  137
+//   50432x384x1536, residual      126   99  110
+//   25216x1024x4096               199  211  225
+//   25216x768x2560                120   94  108
+//   6304x1024x4096                 85   76   63
 template <typename T, int ACT>
 void run_rows(const Mm& a) {
   if (tiles_of(a, 64, 64) <= 600)
     return launch_mm<T, 64, 64, 64, 2, 2, kRowK, kRowK, 2, 1, kAfterFirst, ACT>(
         a);
-  int64_t t = tiles_of(a, 256, 256);
-  bool filled = (a.N + 255) / 256 * 256 <= a.N + a.N / 5;
-  if (filled && t >= 200 && (a.K >= 512 || t >= 768))
-    return launch_mm<T, 256, 256, 64, 4, 4, kRowK, kRowK, 2, 4, kAfterFirst,
+  auto cost = [&](int q, int p, int one) {
+    int64_t n = (tiles_of(a, q, p) + 255) / 256;
+    return one * n + (p < 256 && n > 1 && n % 2 ? one / 2 : 0);
+  };
+  int64_t big = cost(256, 256, 32), mid = cost(160, 128, 12),
+          low = cost(128, 128, 10);
+  if (mid <= low && mid <= big)
+    return launch_mm<T, 160, 128, 64, 2, 2, kRowK, kRowK, 2, 2, kAfterFirst,
                      ACT>(a);
-  launch_mm<T, 128, 128, 64, 2, 4, kRowK, kRowK, 2, 2, kAfterFirst, ACT>(a);
+  if (low <= big)
+    return launch_mm<T, 128, 128, 64, 2, 4, kRowK, kRowK, 2, 2, kAfterFirst,
+                     ACT>(a);
+  launch_mm<T, 256, 256, 64, 4, 4, kRowK, kRowK, 2, 4, kAfterFirst, ACT>(a);
 }
 
 // Both across the sum (weight gradients), in slabs of it: as many as fill the
@@ -957,8 +943,8 @@ void run_cols(const Mm& a, Split s) {
 }
 
 void check_size(int64_t M, int64_t N, int64_t K) {
-  TORCH_CHECK(M < (int64_t(1) << 31) && N <= kMaxCols && K <= kMaxCols,
-              "linear_act: at most 2^31 rows of ", kMaxCols, " values");
+  TORCH_CHECK(M <= (int64_t(1) << 30) && N <= kMaxCols && K <= kMaxCols,
+              "linear_act: at most 2^30 rows of ", kMaxCols, " values");
 }
 
 }  // namespace
@@ -983,7 +969,7 @@ linear_act_fwd(const at::Tensor& x, const at::Tensor& w,
   c10::DeviceGuard guard(x.device());
   auto st = x.scalar_type();
   Mm a{};
-  at::Tensor b, r, ws;
+  at::Tensor b, r;
   if (bias.has_value()) {
     TORCH_CHECK(bias->dim() == 1 && bias->size(0) == N &&
                     bias->device() == x.device() &&
@@ -1007,7 +993,7 @@ linear_act_fwd(const at::Tensor& x, const at::Tensor& w,
     a.e.res_f32 = r.scalar_type() == at::kFloat;
     ot = r.scalar_type();
   }
-  // few rows without a backward pass to come (in training every sum is the
+  // few outputs without a backward pass to come (in training every sum is the
   // tiles', so that it does not go by what is kept); they need neither
   // alignment nor padding
   int few = keep == 0 && !keep_x ? row_groups(M, N) : 0;
@@ -1021,9 +1007,11 @@ linear_act_fwd(const at::Tensor& x, const at::Tensor& w,
   if (act && keep == 2) std::tie(z, zs) = act8_empty({M, N}, x.options());
   c10::optional<at::Tensor> xc, xs;
   if (keep_x) {
-    std::tie(xc, xs) = act8_empty({M, K}, x.options());
-    a.qcodes = (uint8_t*)xc->data_ptr();
-    a.qscale = (uint8_t*)xs->data_ptr();
+    // a pass of its own, ahead of the product, which then finds x in the last
+    // cache: 50432x384x1536 with a 32-bit residual 42 + 105 us, 50432x1536x384
+    // 13 + 123 (141 the other way round). Coding the staged tiles inside the
+    // product won 2 us more, at the cost of registers in every tile size.
+    std::tie(xc, xs) = act8_quantize(x);
   }
   if (z) a.e.z = z->data_ptr();
   if (zs) a.e.zscale = (uint8_t*)zs->data_ptr();
@@ -1059,8 +1047,8 @@ std::tuple<c10::optional<at::Tensor>, c10::optional<at::Tensor>,
 linear_act_bwd(const at::Tensor& dy_in, const c10::optional<at::Tensor>& z,
                const c10::optional<at::Tensor>& zscale,
                const c10::optional<at::Tensor>& xkept,
-               const c10::optional<at::Tensor>& xscale, const at::Tensor& w, const c10::optional<at::Tensor>& mask,
-               bool want_dx, c10::optional<at::ScalarType> dw_type,
+               const c10::optional<at::Tensor>& xscale, const at::Tensor& w,
+               const c10::optional<at::Tensor>& mask, bool want_dx, c10::optional<at::ScalarType> dw_type,
                c10::optional<at::ScalarType> db_type) {
   TORCH_CHECK(dy_in.is_cuda() && dy_in.dim() == 2 && w.dim() == 2 &&
                   is16(w.scalar_type()) && dy_in.device() == w.device() &&
@@ -1245,7 +1233,7 @@ linear_act_bwd(const at::Tensor& dy_in, const c10::optional<at::Tensor>& z,
     });
     if (join) {
       int64_t n = N * K;
-      unsigned grid = (unsigned)((n + kBlock * 8 - 1) / (kBlock * 8));
+      unsigned grid = grid_of((n + kBlock * 8 - 1) / (kBlock * 8), kBlock);
       const float* mp = m.defined() ? m.data_ptr<float>() : nullptr;
       const float* pp = part2.data_ptr<float>();
       if (*dw_type == at::kFloat)
