@@ -319,3 +319,25 @@ def test_two_streams_and_a_graph():
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(u, v) for u, v in zip(out, want))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,C", [(12608, 384), (700, 20000)])
+def test_codes_are_those_of_the_formula(rows, C):
+    """A code is the one nearest to the formula's value but for one in a
+    million. The row's scale is off by half of what the sum's parts of 8 are
+    (2^-24 at most each, as often up as down, and 48 of them or more to a
+    row): some 2e-9 of a value, and the edges between codes are 1/12 of it
+    apart: one in ten million or fewer."""
+    x, r, w, _, _ = make(rows, C, BF16, F32, BF16, "cuda")
+    _, h, kept = add_rms_norm(x, r, w, keep="e4m3")
+    h = h.double()
+    y = h / (h.square().mean(-1, keepdim=True) + 1e-6).sqrt() * w.double()
+    scale = torch.exp2(kept.scales.view(torch.uint8).double() - 127)
+    scale = scale.repeat_interleave(32, -1)[:, :C]
+    v = y / scale
+    step = torch.exp2(v.abs().log2().floor().clamp(min=-6) - 3)
+    want = torch.round(v / step) * step
+    got = kept.dequantize(F32).double() / scale
+    assert (got != want).sum() <= 1e-6 * y.numel()
+    assert ((got - want).abs() <= step).all()

@@ -18,9 +18,7 @@
 // two-pass kernels at the end).
 //
 // Bound by memory: 50432 x 768, bf16 x on a 32-bit stream with codes, forward
-// 95 us (5.3 TB/s), backward 126 us (4.9 TB/s); the vectors' sums 5 us. In 32
-// bits about one code in a million is the neighbour of the one that the formula
-// gives (sums and products in 64 would mend that for 116 us forward).
+// 97 us (5.2 TB/s), backward 126 us (4.9 TB/s); the vectors' sums 5 us.
 
 #include <ATen/ATen.h>
 #include <ATen/hip/HIPContext.h>
@@ -41,19 +39,44 @@ namespace {
 // sum over the TPR threads of a row, in every one of them; TPR = 256 joins
 // its four waves through LDS, and `lds` is free again at the next call only
 // after a barrier, which the alternating half provides
-template <int TPR>
-TP_DEVICE float row_sum(float v, float* lds, int& turn) {
+template <int TPR, typename V>
+TP_DEVICE V row_sum(V v, V* lds, int& turn) {
 #pragma unroll
   for (int off = (TPR < kWave ? TPR : kWave) / 2; off > 0; off >>= 1)
     v += __shfl_xor(v, off, kWave);
   if constexpr (TPR > kWave) {
-    float* l = lds + (turn & 1) * 4;
+    V* l = lds + (turn & 1) * 4;
     ++turn;
     if ((threadIdx.x & (kWave - 1)) == 0) l[threadIdx.x / kWave] = v;
     __syncthreads();
     v = (l[0] + l[1]) + (l[2] + l[3]);
   }
   return v;
+}
+
+// x^-1/2 in 64 bits, from the estimate by one Newton step
+TP_DEVICE double inv_root(double x) {
+  float f = (float)x;
+  double r = rsqrtf(f);
+  return f > 0.f && f < __builtin_inff() ? r + .5 * r * (1. - x * r * r) : r;
+}
+
+// v r w for codes (r is hi + lo): the products with what each leaves, rounded
+// towards zero with the last bit set where anything is cut off, so that
+// rounding to fewer bits gives what rounding v r w would. Where codes are
+// written a row's sum is joined in 64 bits, too: rounded at every step in 32,
+// one code in two million would be the neighbour of the formula's, a sixteenth
+// of its value off, and so it is one in ten million (2 us of 97 at 50432 x
+// 768).
+TP_DEVICE float scaled(float v, float hi, float lo, float w) {
+#pragma clang fp contract(off)
+  float t = v * hi, e = fmaf(v, lo, fmaf(v, hi, -t));
+  float y = t * w, d = fmaf(e, w, fmaf(t, w, -y));
+  float z = y + d, left = d - (z - y);
+  uint32_t b = __float_as_uint(z), l = __float_as_uint(left);
+  // one step down where what is left points to zero
+  b = left != 0.f ? (b - ((b ^ l) >> 31)) | 1 : b;
+  return fabsf(y) < __builtin_inff() ? __uint_as_float(b) : y;
 }
 
 struct NormFwd {
@@ -64,13 +87,14 @@ struct NormFwd {
   uint8_t *codes, *scales;
   int64_t rows, ldx, ldr;
   int C;
-  float eps;
+  double eps, inv;   // inv: 1 / C
 };
 
 // TX: x; TH: residual and h (x's own type without a residual); TY: y.
 template <typename TX, typename TH, typename TY, int TPR, int NCH>
 __global__ __launch_bounds__(kBlock) void rms_fwd_kernel(NormFwd p) {
   __shared__ float lds[8];
+  __shared__ double lds64[8];
   int turn = 0;
   constexpr int RPB = kBlock / TPR;
   int t = threadIdx.x % TPR;
@@ -83,6 +107,7 @@ __global__ __launch_bounds__(kBlock) void rms_fwd_kernel(NormFwd p) {
     TH* h = (TH*)p.h + row * p.C;
     float v[NCH][8];
     float ss = 0.f;
+    double ss64 = 0.;
 #pragma unroll
     for (int j = 0; j < NCH; ++j) {
       int c = (t + j * TPR) * 8, n = live ? p.C - c : 0;
@@ -94,11 +119,21 @@ __global__ __launch_bounds__(kBlock) void rms_fwd_kernel(NormFwd p) {
         for (int i = 0; i < 8; ++i) v[j][i] = rounded<TH>(v[j][i] + rv[i]);
         store8n(h + c, n, v[j]);
       }
+      float s8 = 0.f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) ss = fmaf(v[j][i], v[j][i], ss);
+      for (int i = 0; i < 8; ++i) s8 = fmaf(v[j][i], v[j][i], s8);
+      ss += s8;
+      if (p.codes) ss64 += s8;
     }
-    ss = row_sum<TPR>(ss, lds, turn);
-    float rstd = rsqrtf(ss / p.C + p.eps);
+    float rstd, low = 0.f;
+    if (p.codes) {
+      double s = row_sum<TPR>(ss64, lds64, turn);
+      s = inv_root(fma(s, p.inv, p.eps));
+      rstd = (float)s;
+      low = (float)(s - rstd);
+    } else {
+      rstd = rsqrtf(row_sum<TPR>(ss, lds, turn) / p.C + (float)p.eps);
+    }
     if (live && t == 0 && p.rstd) p.rstd[row] = rstd;
     TY* y = (TY*)p.y + row * p.C;
 #pragma unroll
@@ -106,12 +141,15 @@ __global__ __launch_bounds__(kBlock) void rms_fwd_kernel(NormFwd p) {
       int c = (t + j * TPR) * 8, n = live ? p.C - c : 0;
       float w[8];
       load8n(p.w + c, n, w);
+      float o[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[j][i] = v[j][i] * rstd * w[i];
-      store8n(y + c, n, v[j]);
+      for (int i = 0; i < 8; ++i)
+        o[i] = p.codes ? scaled(v[j][i], rstd, low, w[i])
+                       : v[j][i] * rstd * w[i];
+      store8n(y + c, n, o);
       if (p.codes) {
         int e;
-        uint2 q = encode8(v[j], e, QuadMax());
+        uint2 q = encode8(o, e, QuadMax());
         if (n > 0) {
           store_codes(p.codes + row * p.C + c, n, q);
           if ((t & 3) == 0)
@@ -254,6 +292,7 @@ __global__ __launch_bounds__(1024) void rms_dw_kernel(
 template <typename TX, typename TH, typename TY>
 __global__ __launch_bounds__(kBlock) void rms_fwd_long_kernel(NormFwd p) {
   __shared__ float lds[8];
+  __shared__ double lds64[8];
   int turn = 0;
   int sblk = (p.C + kBlk - 1) / kBlk;
   int span = (p.C + kBlk - 1) / kBlk * kBlk;   // whole quads
@@ -262,6 +301,7 @@ __global__ __launch_bounds__(kBlock) void rms_fwd_long_kernel(NormFwd p) {
     const TH* r = (const TH*)p.r + row * p.ldr;
     TH* h = (TH*)p.h + row * p.C;
     float ss = 0.f;
+    double ss64 = 0.;
     for (int c = threadIdx.x * 8; c < p.C; c += kBlock * 8) {
       float v[8], rv[8];
       load8n(x + c, p.C - c, v);
@@ -271,11 +311,21 @@ __global__ __launch_bounds__(kBlock) void rms_fwd_long_kernel(NormFwd p) {
         for (int i = 0; i < 8; ++i) v[i] = rounded<TH>(v[i] + rv[i]);
         store8n(h + c, p.C - c, v);
       }
+      float s8 = 0.f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) ss = fmaf(v[i], v[i], ss);
+      for (int i = 0; i < 8; ++i) s8 = fmaf(v[i], v[i], s8);
+      ss += s8;
+      if (p.codes) ss64 += s8;
     }
-    ss = row_sum<kBlock>(ss, lds, turn);
-    float rstd = rsqrtf(ss / p.C + p.eps);
+    float rstd, low = 0.f;
+    if (p.codes) {
+      double s = row_sum<kBlock>(ss64, lds64, turn);
+      s = inv_root(fma(s, p.inv, p.eps));
+      rstd = (float)s;
+      low = (float)(s - rstd);
+    } else {
+      rstd = rsqrtf(row_sum<kBlock>(ss, lds, turn) / p.C + (float)p.eps);
+    }
     if (threadIdx.x == 0 && p.rstd) p.rstd[row] = rstd;
     for (int c = threadIdx.x * 8; c < span; c += kBlock * 8) {
       float v[8], rv[8], w[8];
@@ -288,7 +338,8 @@ __global__ __launch_bounds__(kBlock) void rms_fwd_long_kernel(NormFwd p) {
       }
       load8n(p.w + c, n, w);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = v[i] * rstd * w[i];
+      for (int i = 0; i < 8; ++i)
+        v[i] = p.codes ? scaled(v[i], rstd, low, w[i]) : v[i] * rstd * w[i];
       store8n((TY*)p.y + row * p.C + c, n, v);
       if (p.codes) {
         int e;
@@ -458,7 +509,8 @@ rms_fwd(const at::Tensor& x, const c10::optional<at::Tensor>& residual,
   }
   p.rows = rows;
   p.C = (int)C;
-  p.eps = (float)eps;
+  p.eps = eps;
+  p.inv = 1. / (double)C;
   auto stream = at::hip::getCurrentHIPStream();
   by_types(x.scalar_type(), th, out_dtype, [&](auto a, auto b, auto c) {
     using TX = typename decltype(a)::type;
