@@ -654,36 +654,122 @@ __global__ __launch_bounds__(512) void rows_kernel(Mm a) {
       row < a.M ? a.N - c0 : 0, g == 0, v);
 }
 
-// sum of the slabs of a split product, masked and rounded (14 slabs of 1536 x
-// 384, 37 MB in all: 8 us)
+// The ends of both sums over rows: the dz pass's parts of the bias gradient, 16
+// columns to a block, and the slabs of a split product, masked and rounded, by
+// the blocks behind those. Alone each takes 5 to 8 us, most of it latency (14
+// slabs of 1536 x 384, 37 MB in all, 8).
+struct Join {
+  const float* part;   // (slabs, n)
+  const float* mask;   // n values, or null
+  void* out;
+  int64_t n;
+  int slabs;
+  const float* colpart;   // (rows, C)
+  void* colout;
+  int rows, C, coltype;   // type of colout: 0 float32, 1 bfloat16, 2 float16
+};
 template <typename T>
-__global__ __launch_bounds__(kBlock) void join_kernel(
-    const float* __restrict__ part, const float* __restrict__ mask,
-    T* __restrict__ out, int64_t n, int slabs) {
-  int64_t i = ((int64_t)blockIdx.x * kBlock + threadIdx.x) * 8;
-  int m = (int)min((int64_t)8, n - i);
-  if (m <= 0) return;
-  float s[8];
-  load8n(part + i, m, s);
-  for (int k = 1; k < slabs; ++k) {
-    float v[8];
-    load8n(part + (int64_t)k * n + i, m, v);
+__global__ __launch_bounds__(kBlock) void join_kernel(Join a) {
+  __shared__ float sum[16][17];
+  int first = (int)blockIdx.x - (a.C + 15) / 16;
+  if (first >= 0) {
+    int64_t i = ((int64_t)first * kBlock + threadIdx.x) * 8;
+    int m = (int)min((int64_t)8, a.n - i);
+    if (m <= 0) return;
+    float s[8];
+    load8n(a.part + i, m, s);
+    for (int k = 1; k < a.slabs; ++k) {
+      float v[8];
+      load8n(a.part + (int64_t)k * a.n + i, m, v);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) s[j] += v[j];
-  }
-  if (mask) {
-    float v[8];
-    load8n(mask + i, m, v);
+      for (int j = 0; j < 8; ++j) s[j] += v[j];
+    }
+    if (a.mask) {
+      float v[8];
+      load8n(a.mask + i, m, v);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) s[j] = v[j] != 0.f ? s[j] : 0.f;
+      for (int j = 0; j < 8; ++j) s[j] = v[j] != 0.f ? s[j] : 0.f;
+    }
+    store8n((T*)a.out + i, m, s);
+    return;
   }
-  store8n(out + i, m, s);
+  int k = threadIdx.x / 16, l = threadIdx.x % 16;
+  int c = (int)blockIdx.x * 16 + l;
+  float v = 0.f;
+  if (c < a.C) {
+    const float* p = a.colpart + c;
+    int r = k;
+    for (; r + 7 * 16 < a.rows; r += 8 * 16) {
+      float t[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) t[i] = p[(int64_t)(r + i * 16) * a.C];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v += t[i];
+    }
+    for (; r < a.rows; r += 16) v += p[(int64_t)r * a.C];
+  }
+  sum[k][l] = v;
+  __syncthreads();
+  if (k || c >= a.C) return;
+#pragma unroll
+  for (int i = 1; i < 16; ++i) v += sum[i][l];
+  if (a.coltype == 0)
+    ((float*)a.colout)[c] = v;
+  else if (a.coltype == 1)
+    ((__hip_bfloat16*)a.colout)[c] = from_float<__hip_bfloat16>(v);
+  else
+    ((_Float16*)a.colout)[c] = from_float<_Float16>(v);
+}
+
+// w (N, K), rows ldw apart, to (K, N8) with zeros behind N: 64 x 64 tiles
+// through LDS
+struct Turn {
+  const void* w;
+  void* out;
+  int64_t ldw;
+  int N, K, N8;
+};
+template <typename T>
+TP_DEVICE void turn_tile(const Turn& a, int tile, char* lds) {
+  T(*l)[66] = reinterpret_cast<T(*)[66]>(lds);
+  int tn = (a.N8 + 63) / 64;
+  int n0 = tile % tn * 64, k0 = tile / tn * 64;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    int at = i * kBlock + threadIdx.x, r = at / 8, c = at % 8 * 8;
+    int n = n0 + r;
+    float v[8];
+    load8n((const T*)a.w + (int64_t)n * a.ldw + k0 + c,
+           n < a.N ? a.K - k0 - c : 0, v);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) l[c + j][r] = from_float<T>(v[j]);
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    int at = i * kBlock + threadIdx.x, r = at / 8, c = at % 8 * 8;
+    if (k0 + r >= a.K || n0 + c >= a.N8) continue;
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = to_float<T>(l[r][c + j]);
+    store8((T*)a.out + (int64_t)(k0 + r) * a.N8 + n0 + c, v);
+  }
+}
+int64_t turn_tiles(const Turn& t) {
+  return (int64_t)((t.N8 + 63) / 64) * ((t.K + 63) / 64);
+}
+constexpr int kTurnBytes = 64 * 66 * 2;
+template <typename T>
+__global__ __launch_bounds__(kBlock) void turn_kernel(Turn a) {
+  __shared__ __attribute__((aligned(16))) char lds[kTurnBytes];
+  turn_tile<T>(a, blockIdx.x, lds);
 }
 
 // dz = dy act'(z) and the column sums of dz. 32 threads take 256 neighbouring
 // columns, 8 rows at a time; a block adds its rows in registers and joins them
 // in LDS, so the sums need no atomics and keep their order. Bound by memory:
-// 50432 x 1536 with z in 8 bits 84 us, 4.6 TB/s.
+// 50432 x 1536 with z in 8 bits 84 us, 4.6 TB/s. The blocks behind the rows'
+// turn the weight over meanwhile, which takes 5 us by itself, of latency.
 struct Dz {
   const void* dy;
   const void* z;           // 16-bit values or codes; null without act
@@ -692,16 +778,27 @@ struct Dz {
   float* part;             // (blocks, N); null without a bias
   int64_t M;
   int N, ldz;
+  int rows;                // blocks along M; those behind them turn
+  Turn turn;
 };
 template <typename T, typename TG, int CT>
 __global__ __launch_bounds__(kBlock) void dz_kernel(Dz a) {
   constexpr int RL = kBlock / CT;
+  constexpr int SUM = RL * (CT * 8 + 1) * 4;
+  __shared__ __attribute__((aligned(16))) char
+      lds[SUM > kTurnBytes ? SUM : kTurnBytes];
+  if ((int)blockIdx.y >= a.rows) {
+    int64_t t = (int64_t)(blockIdx.y - a.rows) * gridDim.x + blockIdx.x;
+    if (t < (int64_t)((a.turn.N8 + 63) / 64) * ((a.turn.K + 63) / 64))
+      turn_tile<T>(a.turn, (int)t, lds);
+    return;
+  }
   int c = (blockIdx.x * CT + threadIdx.x % CT) * 8;
   int n = a.N - c, rl = threadIdx.x / CT;
   float s[8] = {};
   if (n > 0) {
     for (int64_t r = (int64_t)blockIdx.y * RL + rl; r < a.M;
-         r += (int64_t)gridDim.y * RL) {
+         r += (int64_t)a.rows * RL) {
       float g[8];
       load8n((const TG*)a.dy + r * a.N + c, n, g);
       if (a.z) {
@@ -723,7 +820,7 @@ __global__ __launch_bounds__(kBlock) void dz_kernel(Dz a) {
     }
   }
   if (!a.part) return;
-  __shared__ float sum[RL][CT * 8 + 1];
+  float(*sum)[CT * 8 + 1] = reinterpret_cast<float(*)[CT * 8 + 1]>(lds);
 #pragma unroll
   for (int i = 0; i < 8; ++i) sum[rl][threadIdx.x % CT * 8 + i] = s[i];
   __syncthreads();
@@ -737,33 +834,6 @@ __global__ __launch_bounds__(kBlock) void dz_kernel(Dz a) {
   }
 }
 
-template <typename TO>
-__global__ __launch_bounds__(1024) void colsum_kernel(
-    const float* __restrict__ part, TO* __restrict__ out, int n, int C) {
-  __shared__ float sum[16][64];
-  int c = blockIdx.x * 64 + (threadIdx.x & 63), k = threadIdx.x >> 6;
-  float v = 0.f;
-  if (c < C) {
-    int r = k;
-    for (; r + 7 * 16 < n; r += 8 * 16) {
-      float t[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) t[i] = part[(int64_t)(r + i * 16) * C + c];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v += t[i];
-    }
-    for (; r < n; r += 16) v += part[(int64_t)r * C + c];
-  }
-  sum[k][threadIdx.x & 63] = v;
-  __syncthreads();
-  if (k == 0 && c < C) {
-#pragma unroll
-    for (int i = 1; i < 16; ++i) v += sum[i][threadIdx.x];
-    out[c] = from_float<TO>(v);
-  }
-}
-
-
 // rows of C values to rows of ldo values (a multiple of 8), zeros behind
 template <typename T>
 __global__ __launch_bounds__(kBlock) void pad_kernel(
@@ -776,35 +846,6 @@ __global__ __launch_bounds__(kBlock) void pad_kernel(
   float v[8];
   load8n(x + row * ldx + c, C - c, v);
   store8(out + (row * cpr) * 8 + c, v);
-}
-
-// w (N, K), rows ldw apart, to (K, N8) with zeros behind N: 64 x 64 tiles
-// through LDS (1536 x 384 5 us, 4096 x 1024 6 us: latency)
-template <typename T>
-__global__ __launch_bounds__(kBlock) void turn_kernel(
-    const T* __restrict__ w, T* __restrict__ out, int64_t ldw, int N, int K,
-    int N8) {
-  __shared__ T tile[64][66];
-  int n0 = blockIdx.x * 64, k0 = blockIdx.y * 64;
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    int at = i * kBlock + threadIdx.x, r = at / 8, c = at % 8 * 8;
-    int n = n0 + r;
-    float v[8];
-    load8n(w + (int64_t)n * ldw + k0 + c, n < N ? K - k0 - c : 0, v);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) tile[c + j][r] = from_float<T>(v[j]);
-  }
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    int at = i * kBlock + threadIdx.x, r = at / 8, c = at % 8 * 8;
-    if (k0 + r >= K || n0 + c >= N8) continue;
-    float v[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = to_float<T>(tile[r][c + j]);
-    store8(out + (int64_t)(k0 + r) * N8 + n0 + c, v);
-  }
 }
 
 bool is16(at::ScalarType t) { return t == at::kBFloat16 || t == at::kHalf; }
@@ -1122,6 +1163,23 @@ linear_act_bwd(const at::Tensor& dy_in, const c10::optional<at::Tensor>& z,
   bool products = want_dx || dw_type.has_value();
   at::Tensor dz = same ? dy : at::empty({products ? M : 0, ldz}, opt), part;
   c10::optional<at::Tensor> dx, dw, db;
+  // w along the sum: turned over first where the product is long enough to
+  // win it back (50432x384x1536 in 128 x 128: 95 us and 5 for the turn, 111
+  // across; 25216x1024x4096: 214 and 6, 282 across)
+  Mm in{};
+  in.M = (int)M;
+  in.N = (int)K;
+  in.K = (int)N;
+  bool long_in = want_dx && tiles_of(in, 64, 64) > 600, turned = long_in;
+  at::Tensor ws, wt;
+  Turn turn{};
+  if (long_in) {
+    ws = K <= 1 || w.stride(1) == 1 ? w : w.contiguous();
+    wt = at::empty({K, ldz}, opt);
+    turn = {ws.data_ptr(), wt.data_ptr(), ws.stride(0), (int)N, (int)K,
+            (int)ldz};
+  }
+  Join end{};
   if ((!same && products) || db_type.has_value()) {
     Dz d{};
     d.dy = dy.data_ptr();
@@ -1152,9 +1210,13 @@ linear_act_bwd(const at::Tensor& dy_in, const c10::optional<at::Tensor>& z,
       part = at::empty({gy, N}, opt.dtype(at::kFloat));
       d.part = part.data_ptr<float>();
     }
+    d.rows = gy;
+    if (turned) d.turn = turn;
+    int64_t more = turned ? (turn_tiles(turn) + strips - 1) / strips : 0;
+    turned = more > 0 && gy + more < 65536;
     by16(st, [&](auto t) {
       using T = decltype(t);
-      dim3 grid(strips, gy);
+      dim3 grid(strips, (unsigned)(gy + (turned ? more : 0)));
       auto s = current();
       if (wide && g32)
         dz_kernel<T, float, 32><<<grid, kBlock, 0, s>>>(d);
@@ -1168,58 +1230,47 @@ linear_act_bwd(const at::Tensor& dy_in, const c10::optional<at::Tensor>& z,
     });
     if (db_type.has_value()) {
       db = at::empty({N}, opt.dtype(*db_type));
-      int grid = (int)((N + 63) / 64);
-      if (*db_type == at::kFloat)
-        colsum_kernel<<<grid, 1024, 0, current()>>>(
-            d.part, db->data_ptr<float>(), gy, (int)N);
-      else
-        by16(*db_type, [&](auto t) {
-          using T = decltype(t);
-          colsum_kernel<<<grid, 1024, 0, current()>>>(
-              d.part, (T*)db->data_ptr(), gy, (int)N);
-        });
-      C10_HIP_KERNEL_LAUNCH_CHECK();
+      end.colpart = d.part;
+      end.colout = db->data_ptr();
+      end.rows = gy;
+      end.C = (int)N;
+      end.coltype = *db_type == at::kFloat ? 0 : *db_type == at::kBFloat16 ? 1
+                                                                          : 2;
     }
+  } else {
+    turned = false;
   }
   if (want_dx) {
     dx = at::empty({M, K}, opt);
-    Mm a{};
-    a.q = (const char*)dz.data_ptr();
-    a.ldq = ldz * 2;
-    a.nq = a.M = (int)M;
-    a.N = (int)K;
-    a.K = (int)N;
-    a.e.out = dx->data_ptr();
-    // w along the sum: turned over first where the product is long enough to
-    // win it back (50432x384x1536 in 128 x 128: 95 us and 5 for the turn, 111
-    // across; 25216x1024x4096: 214 and 6, 282 across)
-    if (tiles_of(a, 64, 64) > 600) {
-      auto ws = K <= 1 || w.stride(1) == 1 ? w : w.contiguous();
-      auto wt = at::empty({K, ldz}, opt);
+    in.q = (const char*)dz.data_ptr();
+    in.ldq = ldz * 2;
+    in.nq = (int)M;
+    in.e.out = dx->data_ptr();
+    if (long_in) {
+      in.p = (const char*)wt.data_ptr();
+      in.ldp = ldz * 2;
+      in.np = (int)K;
       by16(st, [&](auto t) {
         using T = decltype(t);
-        turn_kernel<T><<<dim3((unsigned)((ldz + 63) / 64),
-                              (unsigned)((K + 63) / 64)),
-                         kBlock, 0, current()>>>(
-            (const T*)ws.data_ptr(), (T*)wt.data_ptr(), ws.stride(0), (int)N,
-            (int)K, (int)ldz);
-        C10_HIP_KERNEL_LAUNCH_CHECK();
-        a.p = (const char*)wt.data_ptr();
-        a.ldp = ldz * 2;
-        a.np = (int)K;
-        run_rows<T, kNoAct>(a);
+        if (!turned) {
+          turn_kernel<T><<<grid_of(turn_tiles(turn), kBlock), kBlock, 0,
+                           current()>>>(turn);
+          C10_HIP_KERNEL_LAUNCH_CHECK();
+        }
+        run_rows<T, kNoAct>(in);
       });
     } else {
       auto wl = loadable(w);
-      a.p = (const char*)wl.data_ptr();
-      a.ldp = row_bytes(wl);
-      a.np = (int)wl.size(1);
+      in.p = (const char*)wl.data_ptr();
+      in.ldp = row_bytes(wl);
+      in.np = (int)wl.size(1);
       by16(st, [&](auto t) {
         launch_mm<decltype(t), 64, 64, 64, 2, 2, kRowK, kColK, 2, 1,
-                  kAfterFirst>(a);
+                  kAfterFirst>(in);
       });
     }
   }
+  at::Tensor part2, m;   // until the last launch
   if (dw_type.has_value()) {
     dw = at::empty({N, K}, opt.dtype(*dw_type));
     Mm a{};
@@ -1256,7 +1307,6 @@ linear_act_bwd(const at::Tensor& dy_in, const c10::optional<at::Tensor>& z,
       a.ldp = row_bytes(xl);
       a.np = (int)xl.size(1);
     }
-    at::Tensor m;
     if (mask.has_value()) {
       TORCH_CHECK(mask->numel() == N * K && mask->scalar_type() == at::kFloat,
                   "linear_act_bwd: float32 mask of w's shape");
@@ -1265,7 +1315,6 @@ linear_act_bwd(const at::Tensor& dy_in, const c10::optional<at::Tensor>& z,
     Split split = split_of(a);
     int slabs = split.slabs;
     bool join = slabs > 1 || *dw_type != st;
-    at::Tensor part2;
     if (join) {
       part2 = at::empty({slabs, N, K}, opt.dtype(at::kFloat));
       a.e.out = part2.data_ptr();
@@ -1282,21 +1331,24 @@ linear_act_bwd(const at::Tensor& dy_in, const c10::optional<at::Tensor>& z,
         run_cols<T, kColK>(a, split);
     });
     if (join) {
-      int64_t n = N * K;
-      unsigned grid = grid_of((n + kBlock * 8 - 1) / (kBlock * 8), kBlock);
-      const float* mp = m.defined() ? m.data_ptr<float>() : nullptr;
-      const float* pp = part2.data_ptr<float>();
-      if (*dw_type == at::kFloat)
-        join_kernel<<<grid, kBlock, 0, current()>>>(
-            pp, mp, dw->data_ptr<float>(), n, slabs);
-      else
-        by16(*dw_type, [&](auto t) {
-          using T = decltype(t);
-          join_kernel<<<grid, kBlock, 0, current()>>>(
-              pp, mp, (T*)dw->data_ptr(), n, slabs);
-        });
-      C10_HIP_KERNEL_LAUNCH_CHECK();
+      end.part = part2.data_ptr<float>();
+      end.mask = m.defined() ? m.data_ptr<float>() : nullptr;
+      end.out = dw->data_ptr();
+      end.n = N * K;
+      end.slabs = slabs;
     }
+  }
+  if (end.n || end.C) {
+    unsigned grid = grid_of(
+        (end.n + kBlock * 8 - 1) / (kBlock * 8) + (end.C + 15) / 16, kBlock);
+    auto s = current();
+    if (!end.n || *dw_type == at::kFloat)
+      join_kernel<float><<<grid, kBlock, 0, s>>>(end);
+    else
+      by16(*dw_type, [&](auto t) {
+        join_kernel<decltype(t)><<<grid, kBlock, 0, s>>>(end);
+      });
+    C10_HIP_KERNEL_LAUNCH_CHECK();
   }
   return {dx, dw, db};
 }
