@@ -200,6 +200,26 @@ def test_larger(M, K, N, act, keep):
     check(make(M, K, N, res=F32, dev="cuda"), BF16, act, keep)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("bias", [None, F32])
+@pytest.mark.parametrize("res", [None, BF16, F32])
+@pytest.mark.parametrize("M,K,N", [(2000, 2048, 1000), (20000, 200, 40),
+                                   (9000, 384, 1536), (41000, 66, 1)])
+def test_weight_turned_over(M, K, N, res, bias):
+    """Input gradients long enough for it, with a dz pass that does it on the
+    way and without one, and narrow outputs."""
+    check(make(M, K, N, BF16, res, "cuda", bias=bias), BF16, None, None)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("db", [BF16, FP16, F32])
+@pytest.mark.parametrize("dw", [BF16, FP16, F32])
+def test_gradient_types(db, dw):
+    for t in (BF16, FP16):
+        check(make(700, 100, 300, t, t, "cuda", bias=db if db in (t, F32)
+                   else t, weight=dw), t, "gelu", "e4m3")
+
+
 @pytest.mark.parametrize("dev", DEVICES)
 def test_strides_and_leading_dimensions(dev):
     d = make(24, 80, 40, BF16, F32, dev)

@@ -765,11 +765,14 @@ __global__ __launch_bounds__(kBlock) void turn_kernel(Turn a) {
   turn_tile<T>(a, blockIdx.x, lds);
 }
 
-// dz = dy act'(z) and the column sums of dz. 32 threads take 256 neighbouring
-// columns, 8 rows at a time; a block adds its rows in registers and joins them
-// in LDS, so the sums need no atomics and keep their order. Bound by memory:
-// 50432 x 1536 with z in 8 bits 84 us, 4.6 TB/s. The blocks behind the rows'
-// turn the weight over meanwhile, which takes 5 us by itself, of latency.
+// dz = dy act'(z), rounded to the products' 16 bits (matrix instructions take
+// no more of them at that rate; it adds as much to a gradient's error as the
+// rounding of the gradient itself), and the column sums of dz, unrounded. 32
+// threads take 256 neighbouring columns, 8 rows at a time; a block adds its
+// rows in registers and joins them in LDS, so the sums need no atomics and keep
+// their order. Bound by memory: 50432 x 1536 with z in 8 bits 84 us, 4.6 TB/s.
+// The blocks behind the rows' turn the weight over meanwhile, which takes 5 us
+// by itself, of latency.
 struct Dz {
   const void* dy;
   const void* z;           // 16-bit values or codes; null without act
