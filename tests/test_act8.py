@@ -278,7 +278,21 @@ def test_refusals():
     with pytest.raises(ValueError):
         dequantize_act8(Act8(k.codes[:2], k.scales))
     with pytest.raises(ValueError):
+        dequantize_act8(Act8(k.codes[0, 0], k.scales[0, 0]))
+    with pytest.raises(ValueError):
         act8.check_act8(k, like=x[:, :32])
+
+
+@pytest.mark.gpu
+def test_refusals_on_a_gpu():
+    k = quantize_act8(torch.randn(4, 64, device="cuda"))
+    with pytest.raises(TypeError):
+        dequantize_act8(Act8(k.codes.view(torch.uint8), k.scales))
+    for bad in (Act8(k.codes, k.scales[:, :1]), Act8(k.codes[:2], k.scales),
+                Act8(k.codes, k.scales.cpu()), Act8(k.codes.cpu(), k.scales),
+                Act8(k.codes[0, 0], k.scales[0, 0])):
+        with pytest.raises(ValueError):
+            dequantize_act8(bad)
 
 
 @pytest.mark.gpu

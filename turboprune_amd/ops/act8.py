@@ -72,10 +72,14 @@ def dequantize_act8(kept: Act8, dtype: torch.dtype = torch.bfloat16
     """The values that ``kept`` stands for."""
     if dtype not in _FLOATS:
         raise TypeError(f"dtype={dtype}: float32, bfloat16 or float16")
+    codes, scales = kept
+    if _backend.use_native(codes, scales):
+        try:
+            return _backend.extension().act8_dequantize(codes, scales, dtype)
+        except RuntimeError:
+            check_act8(kept)     # which says what is wrong with the arguments
+            raise
     check_act8(kept)
-    if _backend.use_native(kept.codes, kept.scales):
-        return _backend.extension().act8_dequantize(kept.codes, kept.scales,
-                                                    dtype)
     return _dequantize_plain(kept, dtype)
 
 
@@ -87,8 +91,10 @@ def check_act8(kept: Act8, like: Optional[torch.Tensor] = None) -> None:
         raise TypeError("kept: float8_e4m3fn codes and float8_e8m0fnu "
                         f"scales expected, not {codes.dtype} and "
                         f"{scales.dtype}")
+    if codes.dim() < 1:
+        raise ValueError("kept: codes of at least one dimension")
     want = codes.shape[:-1] + (-(-codes.shape[-1] // BLOCK),)
-    if codes.dim() < 1 or scales.shape != want:
+    if scales.shape != want:
         raise ValueError(f"kept: scales of shape {tuple(want)} expected for "
                          f"codes of {tuple(codes.shape)}, not "
                          f"{tuple(scales.shape)}")
