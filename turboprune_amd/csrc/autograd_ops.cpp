@@ -171,7 +171,9 @@ struct LinearAct : Function<LinearAct> {
     d["w"] = weight.sizes();
     auto sizes = x.sizes().vec();
     sizes.back() = N;
-    return y.view(sizes);
+    // not view(): autograd forbids changing a view that a node hands out, and
+    // nothing else holds y
+    return at::_unsafe_view(y, sizes);
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     only_once();
@@ -351,7 +353,8 @@ at::Tensor masked_linear_act(
         r.defined() ? OptTensor(r.dim() == 2 ? r : r.reshape({-1, N}))
                     : OptTensor(),
         act, 0, false);
-    return x.dim() == 2 ? std::get<0>(o) : std::get<0>(o).view(out_sizes);
+    return x.dim() == 2 ? std::get<0>(o)
+                        : at::_unsafe_view(std::get<0>(o), out_sizes);
   }
   return LinearAct::apply(x, w, weight, mask, as_opt(bias), residual, act,
                           keep, codes, scales);

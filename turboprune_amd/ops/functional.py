@@ -316,7 +316,8 @@ def masked_linear_act(x: torch.Tensor, weight: torch.Tensor,
                                    codes, scales)
     else:
         y = _linear_act_fwd_plain(x2, w, bias, r2, act, 0)[0]
-    return y if x.dim() == 2 else y.reshape(lead + (N,))
+    # no view: one made without gradients could not be changed in place later
+    return y if x.dim() == 2 else torch.ops.aten._unsafe_view(y, lead + (N,))
 
 
 def _masked_compute(weight, mask, dtype):
