@@ -1,0 +1,158 @@
+"""The operators with nodes of their own under torch.jit.trace: a traced
+function has to compute them from its own inputs, not to hand out what the
+recorded call had allocated."""
+
+import pytest
+import torch
+
+from turboprune_amd.models.deit import VisionTransformer
+from turboprune_amd.ops import functional as TF
+from turboprune_amd.ops.act8 import (Act8, dequantize_act8, quantize_act8)
+from turboprune_amd.ops.mask_layers import masked_modules
+from turboprune_amd.ops.norm_act import add_rms_norm, gelu
+
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+F32, BF16 = torch.float32, torch.bfloat16
+
+pytestmark = pytest.mark.filterwarnings("ignore")
+
+
+def data(dev, seed, lead=(5, 7)):
+    g = torch.Generator().manual_seed(seed)
+    d = {"x": torch.randn(*lead, 64, generator=g).to(BF16),
+         "r": torch.randn(*lead, 64, generator=g),
+         "nw": torch.rand(64, generator=g) + 0.5,
+         "w": torch.randn(48, 64, generator=g) / 8,
+         "m": (torch.rand(48, 64, generator=g) < 0.7).float(),
+         "b": torch.randn(48, generator=g),
+         "r2": torch.randn(*lead, 48, generator=g)}
+    return {k: v.to(dev) for k, v in d.items()}
+
+
+def norm(d):
+    y, h, _ = add_rms_norm(d["x"], d["r"], d["nw"])
+    return y, h
+
+
+def norm_kept(d):
+    y, h, kept = add_rms_norm(d["x"], d["r"], d["nw"], keep="e4m3")
+    return y, h, kept.dequantize(F32)
+
+
+def norm_alone(d):
+    y, h, kept = add_rms_norm(d["r"], None, d["nw"], keep="e4m3",
+                              out_dtype=BF16)
+    return y, kept.dequantize(BF16)
+
+
+def linear(d):
+    return (TF.masked_linear_act(d["x"], d["w"], d["m"], d["b"], d["r2"],
+                                 "gelu", compute_dtype=BF16, keep="e4m3"),)
+
+
+def linear_16(d):
+    return (TF.masked_linear_act(d["x"], d["w"], d["m"], act="gelu",
+                                 compute_dtype=BF16),)
+
+
+def linear_half(d):
+    return (TF.masked_linear_act(d["r"], d["w"], d["m"], d["b"],
+                                 compute_dtype=torch.float16),)
+
+
+def linear_without_mask(d):
+    return (TF.masked_linear_act(d["x"][0, 0], d["w"], None, d["b"],
+                                 d["r2"][0, 0], compute_dtype=BF16),)
+
+
+def gelu_kept(d):
+    return (gelu(d["x"], keep="e4m3"),)
+
+
+def run(d):
+    """The operators together, as a transformer's MLP has them."""
+    y, h, kept = add_rms_norm(d["x"], d["r"], d["nw"], keep="e4m3")
+    z = TF.masked_linear_act(y, d["w"], d["m"], d["b"], act="gelu",
+                             compute_dtype=BF16, keep="e4m3", kept=kept)
+    return (TF.masked_linear_act(z, d["w"].t(), d["m"].t(), residual=h,
+                                 compute_dtype=BF16, keep="e4m3"), h)
+
+
+def codes(d):
+    k = quantize_act8(d["r"])
+    return (dequantize_act8(Act8(k.codes, k.scales), BF16),)
+
+
+# torch cannot record the plain form's reading of bits as another type, so
+# what writes or reads codes is traced on a GPU only
+PLAIN = [norm, linear_16, linear_half, linear_without_mask]
+OPS = PLAIN + [norm_kept, norm_alone, linear, gelu_kept, run]
+
+
+def on_devices(ops):
+    return [pytest.param("cpu", op, id=f"cpu-{op.__name__}") for op in ops
+            if op in PLAIN] + \
+        [pytest.param("cuda", op, id=f"cuda-{op.__name__}",
+                      marks=pytest.mark.gpu) for op in ops]
+
+
+def traced(op, d):
+    names = list(d)
+    return torch.jit.trace(lambda *a: op(dict(zip(names, a))),
+                           tuple(v.detach() for v in d.values()))
+
+
+@pytest.mark.parametrize("dev,op", on_devices(OPS + [codes]))
+def test_traced_without_gradients(dev, op):
+    with torch.no_grad():
+        f = traced(op, data(dev, 0))
+        for seed in (1, 2):
+            d = data(dev, seed)
+            got, want = f(*d.values()), op(d)
+            for g, w in zip(got, want):
+                # few rows are added in another order where no gradient is
+                # to come, which a trace does not know
+                assert (g.double() - w.double()).abs().max() <= 2.0 ** -7 * (
+                    1 + w.double().abs().max())
+                assert g.dtype == w.dtype and g.shape == w.shape
+
+
+@pytest.mark.parametrize("dev,op", on_devices(OPS))
+def test_traced_with_gradients(dev, op):
+    d = data(dev, 0)
+    names = list(d)
+    ones = tuple(v.requires_grad_(k != "m") for k, v in d.items())
+    f = torch.jit.trace(lambda *a: op(dict(zip(names, a))), ones,
+                        check_trace=False)
+    for seed in (1, 2):
+        d = data(dev, seed)
+        leaves = [v.requires_grad_() for k, v in d.items() if k != "m"]
+        dys = None
+        both = []
+        for call in (lambda: op(d), lambda: f(*d.values())):
+            out = [o for o in call() if o.requires_grad]
+            torch.manual_seed(seed)
+            dys = dys or [torch.randn_like(o) for o in out]
+            both.append([o.detach() for o in out] + list(torch.autograd.grad(
+                out, leaves, dys, allow_unused=True)))
+        for p, q in zip(*both):
+            assert (p is None) == (q is None)
+            assert p is None or torch.equal(p, q)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("kw", [{"fused": True}, {"norm": "rms"}], ids=str)
+def test_traced_model(dev, kw):
+    torch.manual_seed(0)
+    m = VisionTransformer(img_size=32, patch_size=8, embed_dim=96, depth=2,
+                          num_heads=3, num_classes=10, **kw).to(dev).eval()
+    for _, layer in masked_modules(m):
+        layer.enable_cache(BF16)
+    for p in m.parameters():
+        p.requires_grad_(False)
+    xs = [torch.randn(2, 3, 32, 32, device=dev) for _ in range(3)]
+    with torch.no_grad(), torch.autocast(dev, BF16, cache_enabled=False):
+        f = torch.jit.trace(m, xs[0])
+        for x in xs[1:]:
+            a, b = f(x).float(), m(x).float()
+            assert (a - b).norm() <= 2.0 ** -5 * b.norm()

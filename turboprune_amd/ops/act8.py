@@ -63,8 +63,39 @@ def quantize_act8(x: torch.Tensor) -> Act8:
         raise ValueError("quantize_act8: a tensor of at least one dimension")
     x = x.detach()
     if _backend.use_native(x):
-        return Act8(*_backend.extension().act8_quantize(x))
+        return Act8(*(_QuantizeFn.apply(x) if torch.jit.is_tracing()
+                      else _backend.extension().act8_quantize(x)))
     return _quantize_plain(x)
+
+
+class _QuantizeFn(torch.autograd.Function):
+    """A native call as one node of a trace, without gradients: a trace records
+    the allocation of such a call's outputs, but not the kernel that fills
+    them, and a Function as a whole."""
+
+    @staticmethod
+    def forward(ctx, x):
+        codes, scales = _backend.extension().act8_quantize(x)
+        ctx.mark_non_differentiable(codes, scales)
+        return codes, scales
+
+    @staticmethod
+    def backward(ctx, *_):
+        return None
+
+
+class _DequantizeFn(torch.autograd.Function):
+    """The same for the way back."""
+
+    @staticmethod
+    def forward(ctx, codes, scales, dtype):
+        values = _dequantize_native(codes, scales, dtype)
+        ctx.mark_non_differentiable(values)
+        return values
+
+    @staticmethod
+    def backward(ctx, _):
+        return None, None, None
 
 
 def dequantize_act8(kept: Act8, dtype: torch.dtype = torch.bfloat16
@@ -72,15 +103,20 @@ def dequantize_act8(kept: Act8, dtype: torch.dtype = torch.bfloat16
     """The values that ``kept`` stands for."""
     if dtype not in _FLOATS:
         raise TypeError(f"dtype={dtype}: float32, bfloat16 or float16")
-    codes, scales = kept
-    if _backend.use_native(codes, scales):
-        try:
-            return _backend.extension().act8_dequantize(codes, scales, dtype)
-        except RuntimeError:
-            check_act8(kept)     # which says what is wrong with the arguments
-            raise
+    if _backend.use_native(*kept):
+        return (_DequantizeFn.apply if torch.jit.is_tracing()
+                else _dequantize_native)(*kept, dtype)
     check_act8(kept)
     return _dequantize_plain(kept, dtype)
+
+
+def _dequantize_native(codes, scales, dtype):
+    try:
+        return _backend.extension().act8_dequantize(codes, scales, dtype)
+    except RuntimeError:
+        # which says what is wrong with the arguments
+        check_act8(Act8(codes, scales))
+        raise
 
 
 def check_act8(kept: Act8, like: Optional[torch.Tensor] = None) -> None:

@@ -147,8 +147,9 @@ ACTS = (None, "gelu")
 
 class _MaskedLinearAct(torch.autograd.Function):
     """One node from the raw weight: product, bias, activation and residual
-    forward; dx, masked dw, db and dresidual backward. The plain form, for CPU
-    tensors; on a GPU the node is the extension's."""
+    forward; dx, masked dw, db and dresidual backward. The node for CPU tensors,
+    in the plain form, and for torch.jit.trace; on a GPU the node is else the
+    extension's."""
 
     @staticmethod
     def forward(ctx, x, w, weight, mask, bias, residual, act, keep, codes,
@@ -156,11 +157,12 @@ class _MaskedLinearAct(torch.autograd.Function):
         # the pre-activation is needed by the slope, the input only by dw
         need = ctx.needs_input_grad
         need_x, need_z = need[2], need[0] or need[2] or need[4]
-        if keep is not None and codes is None and need_x:
-            codes, scales = act8.quantize_act8(x)
-        y, z, zs = _linear_act_fwd_plain(
+        keep_x = keep is not None and codes is None and need_x
+        y, z, zs, xc, xs = _linear_act_fwd(
             x, w, bias, residual, act,
-            0 if not need_z else 1 if keep is None else 2)
+            0 if not need_z else 1 if keep is None else 2, keep_x)
+        if keep_x:
+            codes, scales = xc, xs
         kept = (None, None) if not need_x else \
             (x, None) if keep is None else (codes, scales)
         ctx.save_for_backward(w, z, zs, *kept, mask if need_x else None)
@@ -175,7 +177,9 @@ class _MaskedLinearAct(torch.autograd.Function):
         need = ctx.needs_input_grad
         dx = dw = db = None
         if need[0] or need[2] or need[4]:
-            dx, dw, db = _linear_act_bwd_plain(
+            bwd = _backend.extension().linear_act_bwd \
+                if _backend.use_native(w) else _linear_act_bwd_plain
+            dx, dw, db = bwd(
                 dy, z, zs, xk, xs, w, mask, need[0],
                 ctx.weight[0] if need[2] else None,
                 ctx.bias if need[4] else None)
@@ -183,6 +187,15 @@ class _MaskedLinearAct(torch.autograd.Function):
             dw = dw.reshape(ctx.weight[1])
         return (dx, None, dw, None, db, dy if need[5] else None, None, None,
                 None, None)
+
+
+def _linear_act_fwd(x, w, bias, residual, act, keep, keep_x):
+    """(y, z, its scales, x's codes, their scales)."""
+    if _backend.use_native(x):
+        return _backend.extension().linear_act_fwd(
+            x, w, bias, residual, act is not None, keep, keep_x)
+    return (*_linear_act_fwd_plain(x, w, bias, residual, act, keep),
+            *(act8.quantize_act8(x) if keep_x else (None, None)))
 
 
 def _linear_act_fwd_plain(x, w, bias, residual, act, keep):
@@ -250,7 +263,9 @@ def masked_linear_act(x: torch.Tensor, weight: torch.Tensor,
     ``add_rms_norm`` hands it on. The weight's gradient is masked and has the
     weight's type.
     """
-    if _backend.use_native(x):
+    native = _backend.use_native(x)
+    tracing = torch.jit.is_tracing()
+    if native and not tracing:
         codes, scales = kept if kept is not None else (None, None)
         return _backend.extension().masked_linear_act(
             x, weight, mask, bias, residual, act, cache, compute_dtype, keep,
@@ -286,9 +301,12 @@ def masked_linear_act(x: torch.Tensor, weight: torch.Tensor,
         ct = compute_dtype or (weight.dtype if weight.dtype != torch.float32
                                else x.dtype)
         with torch.no_grad():
-            w = _masked_compute(weight, mask, ct)
+            w = _masked_compute(weight.detach(), mask, ct)
     ct = w.dtype
     act8.check_float("the compute type", w)
+    if native and ct == torch.float32:
+        raise TypeError("masked_linear_act computes in bfloat16 or float16 on "
+                        "a GPU")
     if residual is not None and residual.dtype not in (ct, torch.float32):
         raise TypeError(f"masked_linear_act: residual in {ct} or float32 "
                         f"expected, not {residual.dtype}")
@@ -306,7 +324,7 @@ def masked_linear_act(x: torch.Tensor, weight: torch.Tensor,
         residual.reshape(-1, N)
     if x2.numel() == 0 or N == 0:
         y = _linear_of_nothing(x2, weight, bias, r2, ct)
-    elif torch.is_grad_enabled() and any(
+    elif native or torch.is_grad_enabled() and any(
             t is not None and t.requires_grad
             for t in (x, weight, bias, residual)):
         codes, scales = (None, None) if kept is None else \
@@ -316,8 +334,12 @@ def masked_linear_act(x: torch.Tensor, weight: torch.Tensor,
                                    codes, scales)
     else:
         y = _linear_act_fwd_plain(x2, w, bias, r2, act, 0)[0]
+    if x.dim() == 2:
+        return y
+    if tracing:                       # the sizes are variables of the trace
+        return y.reshape(lead + (N,))
     # no view: one made without gradients could not be changed in place later
-    return y if x.dim() == 2 else torch.ops.aten._unsafe_view(y, lead + (N,))
+    return torch.ops.aten._unsafe_view(y, lead + (N,))
 
 
 def _masked_compute(weight, mask, dtype):
@@ -325,6 +347,8 @@ def _masked_compute(weight, mask, dtype):
         return weight.to(dtype)
     if weight.dtype == torch.float32 and dtype in (torch.float32,
                                                    torch.bfloat16):
+        if torch.jit.is_tracing():
+            return MaskedWeight.apply(weight, mask, None, dtype)
         return mask_apply(weight, mask, dtype)
     return torch.where(mask != 0, weight, torch.zeros_like(weight)).to(dtype)
 

@@ -73,18 +73,26 @@ class _GeluFn(torch.autograd.Function):
 
 
 class _GeluKeep8Fn(torch.autograd.Function):
-    """The plain form, for CPU tensors; on a GPU the node is the
-    extension's."""
+    """The node for CPU tensors, in the plain form, and for torch.jit.trace; on
+    a GPU the node is else the extension's."""
 
     @staticmethod
     def forward(ctx, x):
-        ctx.save_for_backward(*act8.quantize_act8(x))
-        return gelu_plain(x.float()).to(x.dtype)
+        if _backend.use_native(x):
+            y, *kept = _backend.extension().gelu_keep8_fwd(x)
+        else:
+            y = gelu_plain(x.float()).to(x.dtype)
+            kept = act8.quantize_act8(x)
+        ctx.save_for_backward(*kept)
+        return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        z = act8.dequantize_act8(Act8(*ctx.saved_tensors), torch.float32)
+        codes, scales = ctx.saved_tensors
+        if _backend.use_native(codes):
+            return _backend.extension().gelu_keep8_bwd(codes, scales, dy)
+        z = act8.dequantize_act8(Act8(codes, scales), torch.float32)
         return (dy.float() * gelu_slope(z)).to(dy.dtype)
 
 
@@ -108,7 +116,7 @@ def gelu(x: torch.Tensor, keep: Optional[str] = None) -> torch.Tensor:
     act8.check_keep(keep)
     if keep is None or not (torch.is_grad_enabled() and x.requires_grad):
         return _gelu(x)
-    if _backend.use_native(x):
+    if _backend.use_native(x) and not torch.jit.is_tracing():
         return _backend.extension().gelu_keep8(x)
     act8.check_float("x", x)
     if x.dim() < 1:
@@ -142,13 +150,13 @@ class FusedGELU(nn.Module):
 
 
 class _AddRMSNormFn(torch.autograd.Function):
-    """The plain form, for CPU tensors."""
+    """The node for CPU tensors, in the plain form, and for torch.jit.trace."""
 
     @staticmethod
     def forward(ctx, x, residual, weight, eps, out_dtype, keep):
         ctx.set_materialize_grads(False)
-        y, h, rstd, codes, scales = _rms_fwd_plain(x, residual, weight, eps,
-                                                   out_dtype, keep)
+        y, h, rstd, codes, scales = _rms_fwd(x, residual, weight, eps,
+                                             out_dtype, keep)
         ctx.save_for_backward(x if h is None else h, weight, rstd)
         ctx.x_dtype, ctx.residual = x.dtype, residual is not None
         if codes is not None:
@@ -162,9 +170,17 @@ class _AddRMSNormFn(torch.autograd.Function):
         if dy is None:            # only the sum was used
             dx = None if dh is None else dh.to(ctx.x_dtype)
             return dx, dh, None, None, None, None
-        dx, dr, dw = _rms_bwd_plain(dy, dh, h, weight, rstd, ctx.x_dtype,
-                                    ctx.residual)
+        bwd = _backend.extension().rms_bwd if _backend.use_native(h) \
+            else _rms_bwd_plain
+        dx, dr, dw = bwd(dy, dh, h, weight, rstd, ctx.x_dtype, ctx.residual)
         return dx, dr, dw.to(weight.dtype), None, None, None
+
+
+def _rms_fwd(x, residual, weight, eps, out_dtype, keep):
+    if _backend.use_native(x):
+        return _backend.extension().rms_fwd(x, residual, weight, eps,
+                                            out_dtype, True, keep is not None)
+    return _rms_fwd_plain(x, residual, weight, eps, out_dtype, keep)
 
 
 def _rms_fwd_plain(x, residual, weight, eps, out_dtype, keep):
@@ -211,7 +227,8 @@ def add_rms_norm(x: torch.Tensor, residual: Optional[torch.Tensor],
     in any of the three types. Rows may lie at any distance. Statistics and
     the weight's gradient are summed in float32, in a fixed order.
     """
-    if _backend.use_native(x):
+    native = _backend.use_native(x)
+    if native and not torch.jit.is_tracing():
         y, h, codes, scales = _backend.extension().add_rms_norm(
             x, residual, weight, eps, keep, out_dtype)
         return y, h, None if codes is None else Act8(codes, scales)
@@ -242,7 +259,7 @@ def add_rms_norm(x: torch.Tensor, residual: Optional[torch.Tensor],
         if t is not None and t.device != x.device:
             raise ValueError(f"add_rms_norm: {name} on {t.device}, x on "
                              f"{x.device}")
-    if torch.is_grad_enabled() and (
+    if native or torch.is_grad_enabled() and (
             x.requires_grad or weight.requires_grad
             or (residual is not None and residual.requires_grad)):
         y, h, codes, scales = _AddRMSNormFn.apply(x, residual, weight, eps,
