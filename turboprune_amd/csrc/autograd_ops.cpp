@@ -64,6 +64,15 @@ bool wants_grad(std::initializer_list<const at::Tensor*> ts) {
   return false;
 }
 
+// A dual tensor of forward-mode differentiation need not ask for gradients, and
+// the kernels would drop its tangent.
+void no_tangents(const char* op, std::initializer_list<const at::Tensor*> ts) {
+  for (auto* t : ts)
+    TORCH_CHECK_NOT_IMPLEMENTED(
+        !t->defined() || !t->_fw_grad(0).defined(), op,
+        ": forward-mode derivatives are not available on a GPU");
+}
+
 void only_once() {
   TORCH_CHECK(!at::GradMode::is_enabled(),
               "gradients of gradients are not available for this operator "
@@ -209,6 +218,7 @@ at::Tensor gelu_keep8(const at::Tensor& x) {
   check_float("gelu", "x", x);
   TORCH_CHECK_VALUE(x.dim() >= 1,
                     "gelu(keep=...): a tensor of at least one dimension");
+  no_tangents("gelu", {&x});
   c10::DeviceGuard guard(x.device());
   return GeluKeep8::apply(x);
 }
@@ -231,6 +241,7 @@ std::tuple<at::Tensor, at::Tensor, OptTensor, OptTensor> add_rms_norm(
   check_device(op, "weight", weight, x);
   auto xt = x.scalar_type(), ot = out_dtype.value_or(xt);
   at::Tensor r = or_none(residual);
+  no_tangents(op, {&x, &r, &weight});
   if (residual) {
     TORCH_CHECK_VALUE(r.sizes() == x.sizes(), op, ": residual of shape ",
                       x.sizes(), " expected, not ", r.sizes());
@@ -318,7 +329,8 @@ at::Tensor masked_linear_act(
     want.back() = (K + 31) / 32;
     shape("kept scales", scales, want);
   }
-  at::Tensor w;
+  at::Tensor bias = or_none(bias_in), r = or_none(residual), w;
+  no_tangents(op, {&x_in, &weight, &bias, &r});
   if (cache) {
     w = cache->detach();
   } else {
@@ -332,7 +344,6 @@ at::Tensor masked_linear_act(
               .to(ct);
   }
   auto x = x_in.scalar_type() == ct ? x_in : x_in.to(ct);
-  at::Tensor bias = or_none(bias_in), r = or_none(residual);
   if (bias.defined() && bias.scalar_type() != ct &&
       bias.scalar_type() != at::kFloat)
     bias = bias.to(ct);
