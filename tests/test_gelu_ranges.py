@@ -1,0 +1,94 @@
+"""GELU behind a product over the whole range of what a sum can be."""
+
+import math
+
+import pytest
+import torch
+
+from turboprune_amd.ops import functional as TF
+
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+F32, BF16, FP16 = torch.float32, torch.bfloat16, torch.float16
+
+
+def through(z, t, res, keep, train):
+    """GELU of the values z (N of them, each exact in t) as a product's
+    epilogue gives it: x is a unit vector, z the weight."""
+    N = z.numel()
+    dev = z.device
+    rows = 40 if train else 3
+    x = torch.zeros(rows, 8, device=dev, dtype=t)
+    x[:, 2] = 1
+    w = torch.zeros(N, 8, device=dev)
+    w[:, 2] = z
+    r = None if res is None else torch.zeros(rows, N, device=dev, dtype=res)
+    x.requires_grad_(train)
+    y = TF.masked_linear_act(x, w, None, None, r, "gelu", compute_dtype=t,
+                             keep=keep)
+    assert torch.equal(y, y[:1].expand_as(y))
+    return y[0].detach()
+
+
+def points(t, dev):
+    z = torch.cat((torch.linspace(-40, 40, 4001), torch.linspace(-9, 9, 4001),
+                   -torch.logspace(-3, 2, 500), torch.logspace(-3, 2, 500)))
+    return z.to(t).float().to(dev)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("t", [BF16, FP16])
+@pytest.mark.parametrize("res", [None])
+@pytest.mark.parametrize("keep,train", [(None, False), (None, True),
+                                        ("e4m3", True)])
+def test_every_magnitude(dev, t, res, keep, train):
+    """Relative to the value itself, far tails included. 16-bit results: the
+    short form's tail is off by 5e-6 of itself up to |z| = 4, by 5e-5 up to
+    6.5 and its exponent's roundings by 2^-21 (1 + z^2); behind 6.5, and for
+    32-bit results everywhere, the tail is off by (1.5e-6 + 1e-7 z^2) of
+    itself. z (1 - tail) rounds twice, fp32 ends at 2^-126 (what a product
+    flushes below is at most that), and the type rounds once."""
+    z = points(t, dev)
+    got = through(z, t, res, keep, train).double().cpu()
+    z = z.double().cpu()
+    want = z * 0.5 * torch.special.erfc(-z / math.sqrt(2))
+    tail = z.abs() * 0.5 * torch.special.erfc(z.abs() / math.sqrt(2))
+    rel = 1.5e-6 + 1e-7 * z * z
+    if res is None:
+        short = torch.where(z.abs() <= 4, 5e-6, 5e-5) \
+            + 2.0 ** -21 * (1 + z * z)
+        # above 6.5 the tail is nothing beside z
+        rel = torch.where(z.abs() <= 6.5, short, rel)
+    ot = t if res is None else res
+    tol = tail * rel + want.abs() * (2.0 ** -22 + torch.finfo(ot).eps / 2) \
+        + (2.0 ** -25 if ot == FP16 else 2.0 ** -125)
+    if res is None:
+        tol = tol + torch.where(z > 6.5, 3e-10, 0.0)
+    bad = (got - want).abs() > tol
+    assert not bad.any(), (z[bad][:5], got[bad][:5], want[bad][:5])
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("t", [BF16, FP16])
+@pytest.mark.parametrize("res", [None, F32])
+@pytest.mark.parametrize("train", [False, True])
+def test_infinities(dev, t, res, train):
+    """z Phi(z) at infinity is inf and at -inf inf times 0, no number, as
+    torch's GELU has it; beside them nothing changes."""
+    z = torch.tensor([1., -2., math.inf, -math.inf, math.nan, -7., 8., -8.],
+                     device=dev)
+    N = z.numel()
+    x = torch.zeros(40, 8, device=dev, dtype=t)
+    bias = z.clone()
+    r = None if res is None else torch.zeros(40, N, device=dev)
+    w = torch.zeros(N, 8, device=dev)
+    x.requires_grad_(train)
+    y = TF.masked_linear_act(x, w, None, bias, r, "gelu",
+                             compute_dtype=t).detach()[5].float().cpu()
+    want = torch.nn.functional.gelu(z.double()).cpu()
+    assert torch.equal(y.isnan(), want.isnan())
+    assert y[2] == math.inf
+    fin = want.isfinite()
+    ot = t if res is None else res
+    assert ((y[fin].double() - want[fin]).abs()
+            <= want[fin].abs() * (torch.finfo(ot).eps / 2 + 2e-5)
+            + 2.0 ** -24).all()

@@ -272,8 +272,8 @@ TP_DEVICE float gelu(float z) {
 // bound the epilogue: gelu(z) = max(z, 0) - t Phi(-t), t = |z|, with
 // Phi(-t) = 2^-h(t), h a polynomial (fitted here over [0, 6.5] and exactly 1
 // at 0): 14 instruction slots a value against 25. Off by 5e-6 of t Phi(-t) up
-// to t = 4, by 5e-5 up to 6.5; behind it t stays at 6.5 and the result within
-// 3e-10 of max(z, 0).
+// to t = 4, by 5e-5 up to 6.5. Above 6.5 t stays there and the result within
+// 3e-10 of z; it is not for z below -6.5, where the tail is all there is.
 TP_DEVICE float gelu_short(float z) {
   float t = fminf(fabsf(z), 6.5f);
   float h = 1.7347767879982712e-06f;

@@ -309,6 +309,22 @@ TP_DEVICE void add8(const T* p, int n, float (&v)[8]) {
   for (int i = 0; i < 8; ++i) v[i] += r[i];
 }
 
+// GELU of a lane's 8 values. gelu_short holds from -6.5 on; behind that, and
+// at -inf, the tail is the longer form's. One value in 10^10 of a normal
+// distribution lies there, so a wave seldom takes the branch.
+TP_DEVICE void gelu_all(float (&v)[8]) {
+  float low = v[0];
+#pragma unroll
+  for (int i = 1; i < 8; ++i) low = fminf(low, v[i]);   // passes NaN over
+  if (__builtin_expect(low >= -6.5f || low != low, 1)) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = gelu_short(v[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = gelu(v[i]);
+  }
+}
+
 // v: the sums of 8 neighbouring columns of one row; n of them exist (<= 0:
 // none; FULL: all). The lanes l, l^16, l^32 and l^48 hold one 32-column block.
 // PLAIN: no residual, no mask, 16-bit output, known beforehand (choosing here
@@ -327,9 +343,7 @@ TP_DEVICE void epilogue8(const Epi& e, int64_t at, int64_t blk, int n,
   }
   if constexpr (ACT == kGelu)
     if (e.z) put8<FULL>((T*)e.z + at, n, v);
-  if constexpr (ACT != kNoAct)
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = gelu_short(v[i]);
+  if constexpr (ACT != kNoAct) gelu_all(v);
   if constexpr (PLAIN) {
     put8<FULL>((T*)e.out + at, n, v);
     return;
