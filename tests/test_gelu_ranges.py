@@ -1,4 +1,5 @@
-"""GELU behind a product over the whole range of what a sum can be."""
+"""GELU behind a product over the whole range of what a sum can be, for 16-bit
+and 32-bit results."""
 
 import math
 
@@ -37,7 +38,7 @@ def points(t, dev):
 
 @pytest.mark.parametrize("dev", DEVICES)
 @pytest.mark.parametrize("t", [BF16, FP16])
-@pytest.mark.parametrize("res", [None])
+@pytest.mark.parametrize("res", [None, F32])
 @pytest.mark.parametrize("keep,train", [(None, False), (None, True),
                                         ("e4m3", True)])
 def test_every_magnitude(dev, t, res, keep, train):
@@ -65,6 +66,18 @@ def test_every_magnitude(dev, t, res, keep, train):
         tol = tol + torch.where(z > 6.5, 3e-10, 0.0)
     bad = (got - want).abs() > tol
     assert not bad.any(), (z[bad][:5], got[bad][:5], want[bad][:5])
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_32_bit_results_are_as_close_as_the_plain_form(dev):
+    """The distance from the formula in the mean square over [-9, 9], against
+    that of the function written with erf in 32 bits."""
+    z = torch.linspace(-9, 9, 16384).to(BF16).float().to(dev)
+    got = through(z, BF16, F32, None, True).double().cpu()
+    plain = (0.5 * z * (1 + torch.erf(z * 0.5 ** 0.5))).double().cpu()
+    z = z.double().cpu()
+    want = z * 0.5 * torch.special.erfc(-z / math.sqrt(2))
+    assert (got - want).norm() <= 1.25 * (plain - want).norm()
 
 
 @pytest.mark.parametrize("dev", DEVICES)

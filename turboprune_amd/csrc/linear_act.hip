@@ -311,12 +311,14 @@ TP_DEVICE void add8(const T* p, int n, float (&v)[8]) {
 
 // GELU of a lane's 8 values. gelu_short holds from -6.5 on; behind that, and
 // at -inf, the tail is the longer form's. One value in 10^10 of a normal
-// distribution lies there, so a wave seldom takes the branch.
-TP_DEVICE void gelu_all(float (&v)[8]) {
+// distribution lies there, so a wave seldom takes the branch. 32-bit results
+// (wide) have the longer form throughout: the short one's 8.5e-7 is more than
+// their own rounding.
+TP_DEVICE void gelu_all(float (&v)[8], bool wide) {
   float low = v[0];
 #pragma unroll
   for (int i = 1; i < 8; ++i) low = fminf(low, v[i]);   // passes NaN over
-  if (__builtin_expect(low >= -6.5f || low != low, 1)) {
+  if (!wide && (low >= -6.5f || low != low)) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = gelu_short(v[i]);
   } else {
@@ -343,7 +345,7 @@ TP_DEVICE void epilogue8(const Epi& e, int64_t at, int64_t blk, int n,
   }
   if constexpr (ACT == kGelu)
     if (e.z) put8<FULL>((T*)e.z + at, n, v);
-  if constexpr (ACT != kNoAct) gelu_all(v);
+  if constexpr (ACT != kNoAct) gelu_all(v, !PLAIN && e.out_f32);
   if constexpr (PLAIN) {
     put8<FULL>((T*)e.out + at, n, v);
     return;
