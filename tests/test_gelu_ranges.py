@@ -1,5 +1,6 @@
 """GELU behind a product over the whole range of what a sum can be, for 16-bit
-and 32-bit results."""
+and 32-bit results, and its slope where the kept pre-activation would not fit
+16 bits."""
 
 import math
 
@@ -105,3 +106,23 @@ def test_infinities(dev, t, res, train):
     assert ((y[fin].double() - want[fin]).abs()
             <= want[fin].abs() * (torch.finfo(ot).eps / 2 + 2e-5)
             + 2.0 ** -24).all()
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("keep", [None, "e4m3"])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_pre_activation_beyond_half_precision(dev, keep, sign):
+    """A sum of 10^5 under a float32 residual is a finite output; its slope is
+    1 (0 at -10^5), also where z is kept in float16."""
+    x = torch.full((40, 64), 40.0, device=dev, dtype=FP16).requires_grad_()
+    w = torch.full((24, 64), 40.0 * sign, device=dev)
+    r = torch.ones(40, 24, device=dev)
+    b = torch.zeros(24, device=dev, requires_grad=True)
+    y = TF.masked_linear_act(x, w, None, b, r, "gelu", compute_dtype=FP16,
+                             keep=keep)
+    assert (y == (102401.0 if sign > 0 else 1.0)).all()
+    dy = torch.full_like(y, 2.0 ** -10)
+    dx, db = torch.autograd.grad(y, (x, b), dy)
+    # 24 terms of 40 * 2^-10, 40 of 2^-10: exact
+    assert (dx == (0.9375 if sign > 0 else 0.0)).all()
+    assert (db == (40 * 2.0 ** -10 if sign > 0 else 0.0)).all()

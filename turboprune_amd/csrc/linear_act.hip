@@ -344,7 +344,14 @@ TP_DEVICE void epilogue8(const Epi& e, int64_t at, int64_t blk, int n,
     }
   }
   if constexpr (ACT == kGelu)
-    if (e.z) put8<FULL>((T*)e.z + at, n, v);
+    if (e.z) {
+      // within the finite range: the slope of an fp16 infinity would be NaN
+      // beside a result that is finite in 32 bits
+      float k[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) k[i] = held_in<T>(v[i]);
+      put8<FULL>((T*)e.z + at, n, k);
+    }
   if constexpr (ACT != kNoAct) gelu_all(v, !PLAIN && e.out_f32);
   if constexpr (PLAIN) {
     put8<FULL>((T*)e.out + at, n, v);

@@ -209,8 +209,11 @@ def _linear_act_fwd_plain(x, w, bias, residual, act, keep):
     y = y.to(x.dtype if residual is None else residual.dtype)
     if act is None or keep == 0:
         return y, None, None
-    return (y, z.to(x.dtype), None) if keep == 1 else \
-        (y, *act8.quantize_act8(z))
+    if keep == 2:
+        return y, *act8.quantize_act8(z)
+    if x.dtype == torch.float16:    # an infinity would have no slope
+        z = z.clamp(-65504.0, 65504.0)
+    return y, z.to(x.dtype), None
 
 
 def _linear_act_bwd_plain(dy, z, zs, xk, xs, w, mask, want_dx, dw_type, db_type):
