@@ -125,6 +125,8 @@ linear_act_bwd(const at::Tensor&, const c10::optional<at::Tensor>&,
                const c10::optional<at::Tensor>&, const at::Tensor&,
                const c10::optional<at::Tensor>&, bool,
                c10::optional<at::ScalarType>, c10::optional<at::ScalarType>);
+std::tuple<int64_t, int64_t> linear_act_tile(int64_t, int64_t);
+std::tuple<int64_t, int64_t> linear_act_split(int64_t, int64_t, int64_t);
 }  // namespace turboprune
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -225,6 +227,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         "its scales)");
   m.def("linear_act_bwd", &turboprune::linear_act_bwd,
         "gradients of linear_act_fwd -> (dx, dw, dbias)");
+  m.def("linear_act_tile", &turboprune::linear_act_tile,
+        "(rows, columns) of the tiles that a product of M x N values takes");
+  m.def("linear_act_split", &turboprune::linear_act_split,
+        "(tile, slabs) of the gradient of an N x K weight over M rows");
   m.def("gelu_keep8", &turboprune::gelu_keep8,
         "exact GELU, its input kept in 8 bits (autograd)");
   m.def("add_rms_norm", &turboprune::add_rms_norm,

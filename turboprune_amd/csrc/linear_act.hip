@@ -946,8 +946,11 @@ void launch_mm(Mm a, int slabs = 1) {
   C10_HIP_KERNEL_LAUNCH_CHECK();
 }
 
+int64_t tiles_of(int64_t M, int64_t N, int q, int p) {
+  return (M + q - 1) / q * ((N + p - 1) / p);
+}
 int64_t tiles_of(const Mm& a, int q, int p) {
-  return (int64_t)((a.M + q - 1) / q) * ((a.N + p - 1) / p);
+  return tiles_of(a.M, a.N, q, p);
 }
 
 // Groups of 16 rows that a block of rows_kernel takes, 0: the tiles. Such
@@ -1004,24 +1007,34 @@ void run_few(const Mm& a, int groups) {
 //   25216x1024x4096               199  211  225
 //   25216x768x2560                120   94  108
 //   6304x1024x4096                 85   76   63
-template <typename T, int ACT>
-void run_rows(const Mm& a) {
-  if (tiles_of(a, 64, 64) <= 600)
-    return launch_mm<T, 64, 64, 64, 2, 2, kRowK, kRowK, 2, 1, kAfterFirst, ACT>(
-        a);
+std::tuple<int64_t, int64_t> rows_tile(int64_t M, int64_t N) {
+  if (tiles_of(M, N, 64, 64) <= 600) return {64, 64};
   auto cost = [&](int q, int p, int one) {
-    int64_t n = (tiles_of(a, q, p) + 255) / 256;
+    int64_t n = (tiles_of(M, N, q, p) + 255) / 256;
     return one * n + (p < 256 && n > 1 && n % 2 ? one / 2 : 0);
   };
   int64_t big = cost(256, 256, 32), mid = cost(160, 128, 12),
           low = cost(128, 128, 10);
-  if (mid <= low && mid <= big)
-    return launch_mm<T, 160, 128, 64, 2, 2, kRowK, kRowK, 2, 2, kAfterFirst,
-                     ACT>(a);
-  if (low <= big)
-    return launch_mm<T, 128, 128, 64, 2, 4, kRowK, kRowK, 2, 2, kAfterFirst,
-                     ACT>(a);
-  launch_mm<T, 256, 256, 64, 4, 4, kRowK, kRowK, 2, 4, kAfterFirst, ACT>(a);
+  if (mid <= low && mid <= big) return {160, 128};
+  if (low <= big) return {128, 128};
+  return {256, 256};
+}
+template <typename T, int ACT>
+void run_rows(const Mm& a) {
+  switch (std::get<0>(rows_tile(a.M, a.N))) {
+    case 64:
+      return launch_mm<T, 64, 64, 64, 2, 2, kRowK, kRowK, 2, 1, kAfterFirst,
+                       ACT>(a);
+    case 160:
+      return launch_mm<T, 160, 128, 64, 2, 2, kRowK, kRowK, 2, 2, kAfterFirst,
+                       ACT>(a);
+    case 128:
+      return launch_mm<T, 128, 128, 64, 2, 4, kRowK, kRowK, 2, 2, kAfterFirst,
+                       ACT>(a);
+    default:
+      return launch_mm<T, 256, 256, 64, 4, 4, kRowK, kRowK, 2, 4, kAfterFirst,
+                       ACT>(a);
+  }
 }
 
 // Both across the sum (weight gradients), in slabs of it: as many as fill the
@@ -1067,6 +1080,23 @@ void check_size(int64_t M, int64_t N, int64_t K) {
 }
 
 }  // namespace
+
+// rows and columns of the tiles that a product of M x N values along both rows
+// runs in (few rows without a gradient aside)
+std::tuple<int64_t, int64_t> linear_act_tile(int64_t M, int64_t N) {
+  return rows_tile(M, N);
+}
+// rows and columns of the tiles, and slabs, of the gradient of an N x K weight
+// over M rows
+std::tuple<int64_t, int64_t> linear_act_split(int64_t M, int64_t N, int64_t K) {
+  check_size(M, N, K);
+  Mm a{};
+  a.M = (int)N;
+  a.N = (int)K;
+  a.K = (int)M;
+  Split s = split_of(a);
+  return {s.tile, s.slabs};
+}
 
 // (y, z, scales of z, x's codes, their scales). keep: 0 keeps nothing, 1 the
 // pre-activation in 16 bits, 2 in 8 bits (only with act); keep_x: x in 8 bits.
