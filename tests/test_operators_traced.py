@@ -141,7 +141,8 @@ def test_traced_with_gradients(dev, op):
 
 
 @pytest.mark.parametrize("dev", DEVICES)
-@pytest.mark.parametrize("kw", [{"fused": True}, {"norm": "rms"}], ids=str)
+@pytest.mark.parametrize("kw", [{"fused": True}, {"norm": "rms"},
+                                {"norm": "rms", "keep": "e4m3"}], ids=str)
 def test_traced_model(dev, kw):
     torch.manual_seed(0)
     m = VisionTransformer(img_size=32, patch_size=8, embed_dim=96, depth=2,

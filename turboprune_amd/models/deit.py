@@ -158,9 +158,14 @@ class Block(nn.Module):
             x = x + self.attn.fused(self.norm1(x), keep)
             return self.mlp.fused(self.norm2(x), x, keep)
         # the second norm adds the attention's output to the stream; both hand
-        # their rows on in 8 bits as well, which the next product keeps
-        y, x, kept = self.norm1.add(x, None, keep)
-        y, x, kept = self.norm2.add(self.attn.fused(y, keep, kept), x, keep)
+        # their rows on in 8 bits as well, which the next product keeps for its
+        # weight's gradient, where there will be one
+        def rows(layer):
+            return keep if torch.is_grad_enabled() \
+                and layer.weight.requires_grad else None
+        y, x, kept = self.norm1.add(x, None, rows(self.attn.qkv))
+        y, x, kept = self.norm2.add(self.attn.fused(y, keep, kept), x,
+                                    rows(self.mlp.fc1))
         return self.mlp.fused(y, x, keep, kept)
 
 
