@@ -1,13 +1,110 @@
-"""The fused blocks of the transformer models: what they compute beside what
-their modules' own calls would."""
+"""The fused blocks pass by their modules' calls. What hangs on such a call (a
+hook, another module in a place) has to be honoured all the same."""
 
 import pytest
 import torch
+import torch.nn as nn
 
 from test_deit_kept import step, vit
 from turboprune_amd.ops.norm_act import FusedRMSNorm
 
 DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+KW = [{"fused": True}, {"norm": "rms"}, {"keep": "e4m3"},
+      {"norm": "rms", "keep": "e4m3"}]
+PARTS = ["norm1", "attn", "attn.qkv", "attn.proj", "norm2", "mlp", "mlp.fc1",
+         "mlp.act", "mlp.fc2", "mlp.drop"]
+
+
+def close(a, b, tol):
+    (la, ga), (lb, gb) = a, b
+    assert abs(la - lb) <= tol * (1 + abs(la))
+    for n in ga:
+        assert (ga[n] - gb[n]).norm() <= tol * ga[n].norm() + 1e-9, n
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("kw", KW, ids=str)
+def test_hooks_fire(dev, kw):
+    m = vit(dev, **kw)
+    ref = step(m, dev)
+    for kind in ("register_forward_hook", "register_forward_pre_hook",
+                 "register_full_backward_hook"):
+        for part in PARTS:
+            seen = []
+            mod = m.blocks[1].get_submodule(part)
+            h = getattr(mod, kind)(lambda *a: seen.append(a[0]))
+            got = step(m, dev)
+            # dropout stands behind both products
+            assert seen == [mod] * (1 + (part == "mlp.drop")), (kind, part)
+            h.remove()
+            tol = 1e-5 if dev == "cpu" else 2.0 ** -5
+            close(ref, got, 2.0 ** -3 if "keep" in kw else tol)
+    seen = []
+    h = torch.nn.modules.module.register_module_forward_hook(
+        lambda mod, *a: seen.append(mod))
+    step(m, dev)
+    h.remove()
+    assert all(m.blocks[0].get_submodule(p) in seen for p in PARTS)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_a_hook_changes_the_output(dev):
+    m = vit(dev, norm="rms")
+    plain = step(m, dev)[0]
+    h = m.blocks[0].mlp.fc1.register_forward_hook(lambda *a: a[2] * 0)
+    assert abs(step(m, dev)[0] - plain) > 1e-4
+    h.remove()
+    assert step(m, dev)[0] == plain
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("kw", KW, ids=str)
+def test_replaced_modules(dev, kw):
+    """Another activation, another MLP, another attention, a norm of another
+    kind and a forward method put over a module's own."""
+    def changed(m, how):
+        b = m.blocks[0]
+        if how == "act":
+            b.mlp.act = nn.ReLU()
+        elif how == "mlp":
+            b.mlp = nn.Sequential(nn.LayerNorm(96), nn.Tanh()).to(dev)
+        elif how == "attn":
+            b.attn = nn.Identity()
+        elif how == "norm":
+            b.norm2 = nn.LayerNorm(96).to(dev)
+        elif how == "linear":
+            torch.manual_seed(5)
+            b.mlp.fc2 = nn.Linear(384, 96).to(dev)
+        else:
+            own = b.mlp.fc1.forward
+            b.mlp.fc1.forward = lambda x: own(x) * 0.5
+        return m
+
+    class Unfused(nn.Module):
+        """The block's formula, written with its modules."""
+        def __init__(self, b):
+            super().__init__()
+            self.b = b
+
+        def forward(self, x):
+            b = self.b
+            x = x + b.attn(b.norm1(x))
+            h = b.mlp
+            if hasattr(h, "fc1"):
+                y = h.fc2(h.act(h.fc1(b.norm2(x))))
+            else:
+                y = h(b.norm2(x))
+            return x + y
+
+    for how in ("act", "mlp", "attn", "norm", "linear", "forward"):
+        got = step(changed(vit(dev, **kw), how), dev)
+        ref = vit(dev, **{k: v for k, v in kw.items() if k == "norm"})
+        ref = changed(ref, how)
+        ref.blocks = nn.ModuleList(Unfused(b) for b in ref.blocks)
+        want = step(ref, dev)
+        want = want[0], {n.replace(".b.", "."): g for n, g in want[1].items()}
+        tol = 1e-5 if dev == "cpu" else 2.0 ** -5
+        close(want, got, 2.0 ** -3 if "keep" in kw else tol)
 
 
 @pytest.mark.parametrize("dev", DEVICES)

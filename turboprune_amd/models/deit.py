@@ -18,6 +18,11 @@ epilogues: ``fused=True`` is that alone, ``norm="rms"`` takes root-mean-square
 norms that add the residual on the way, ``keep="e4m3"`` holds what the linear
 layers and the MLP's GELU need for the backward pass in 8 bits. They compute in
 16 bits on a GPU: under autocast or with the layers' caches enabled.
+
+The fused operators pass by their modules' calls. A block with a hook on one of
+its modules, a hook on all modules, or another module in place of one of them
+therefore runs module by module, with the same results up to rounding; of what
+it keeps, only the GELU's input is then in 8 bits.
 """
 
 from __future__ import annotations
@@ -26,9 +31,10 @@ from functools import partial
 
 import torch
 import torch.nn as nn
+from torch.nn.modules.module import _has_any_global_hook
 
 from turboprune_amd.ops.act8 import check_keep
-from turboprune_amd.ops.mask_layers import Conv1dMask, ConvMask
+from turboprune_amd.ops.mask_layers import Conv1dMask, ConvMask, LinearMask
 from turboprune_amd.ops.norm_act import (FusedGELU, FusedLayerNorm,
                                          FusedRMSNorm)
 
@@ -112,10 +118,10 @@ class Attention(nn.Module):
 
 
 class Mlp(nn.Module):
-    def __init__(self, in_features, hidden_features, drop=0.0):
+    def __init__(self, in_features, hidden_features, drop=0.0, keep=None):
         super().__init__()
         self.fc1 = Conv1dMask(in_features, hidden_features, bias=True)
-        self.act = FusedGELU()
+        self.act = FusedGELU(keep)
         self.fc2 = Conv1dMask(hidden_features, in_features, bias=True)
         self.drop = nn.Dropout(drop)
 
@@ -131,6 +137,15 @@ class Mlp(nn.Module):
         return self.fc2.fused(x, residual=residual, keep=keep)
 
 
+def _bare(module: nn.Module, *forwards) -> bool:
+    """Whether a call of the module runs one of these methods and nothing
+    else."""
+    d = module.__dict__
+    return type(module).forward in forwards and "forward" not in d and not (
+        d["_forward_hooks"] or d["_forward_pre_hooks"]
+        or d["_backward_hooks"] or d["_backward_pre_hooks"])
+
+
 class Block(nn.Module):
     def __init__(self, dim, num_heads, mlp_ratio=4.0, qkv_bias=True,
                  drop=0.0, attn_drop=0.0, norm_layer=nn.LayerNorm,
@@ -142,19 +157,35 @@ class Block(nn.Module):
         self.norm1 = norm_layer(dim)
         self.attn = Attention(dim, num_heads, qkv_bias, attn_drop, drop)
         self.norm2 = norm_layer(dim)
-        self.mlp = Mlp(dim, int(dim * mlp_ratio), drop)
+        self.mlp = Mlp(dim, int(dim * mlp_ratio), drop, keep)
 
     def forward(self, x):
-        if self.fused or self.keep is not None \
-                or isinstance(self.norm1, FusedRMSNorm):
-            return self._fused(x)
+        rms = isinstance(self.norm1, FusedRMSNorm)
+        if (self.fused or self.keep is not None or rms) \
+                and self._fusible(rms):
+            return self._fused(x, rms)
         x = x + self.attn(self.norm1(x))
         x = x + self.mlp(self.norm2(x))
         return x
 
-    def _fused(self, x):
+    def _fusible(self, rms: bool) -> bool:
+        """Whether nothing hangs on the calls that ``_fused`` passes by."""
+        a, m = self.attn, self.mlp
+        if _has_any_global_hook() or not (_bare(a, Attention.forward)
+                                          and _bare(m, Mlp.forward)):
+            return False
+        return all(_bare(layer, Conv1dMask.forward, LinearMask.forward)
+                   for layer in (a.qkv, a.proj, m.fc1, m.fc2)) \
+            and (not rms or _bare(self.norm1, FusedRMSNorm.forward)
+                 and _bare(self.norm2, FusedRMSNorm.forward)) \
+            and _bare(m.act, FusedGELU.forward, nn.GELU.forward) \
+            and getattr(m.act, "approximate", "none") == "none" \
+            and getattr(m.act, "keep", None) in (None, self.keep) \
+            and _bare(m.drop, nn.Dropout.forward)
+
+    def _fused(self, x, rms: bool):
         keep = self.keep
-        if not isinstance(self.norm1, FusedRMSNorm):
+        if not rms:
             x = x + self.attn.fused(self.norm1(x), keep)
             return self.mlp.fused(self.norm2(x), x, keep)
         # the second norm adds the attention's output to the stream; both hand
