@@ -1,5 +1,6 @@
 """The fused blocks pass by their modules' calls. What hangs on such a call (a
-hook, another module in a place) has to be honoured all the same."""
+hook, another module in a place, a type that the products do not compute in)
+has to be honoured all the same."""
 
 import pytest
 import torch
@@ -105,6 +106,37 @@ def test_replaced_modules(dev, kw):
         want = want[0], {n.replace(".b.", "."): g for n, g in want[1].items()}
         tol = 1e-5 if dev == "cpu" else 2.0 ** -5
         close(want, got, 2.0 ** -3 if "keep" in kw else tol)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("kw", KW, ids=str)
+def test_float32_training(dev, kw):
+    """Without autocast and caches the products are float32, which the fused
+    ones are not on a GPU; the block runs all the same."""
+    m = vit(dev, **kw)
+    ref = vit("cpu", **{k: v for k, v in kw.items() if k == "norm"})
+    ref.load_state_dict({k: v.cpu() for k, v in m.state_dict().items()})
+    torch.manual_seed(3)
+    x, y = torch.randn(6, 3, 32, 32), torch.randint(0, 10, (6,))
+    out = []
+    for mod, d in ((ref, "cpu"), (m, dev)):
+        loss = nn.functional.cross_entropy(mod(x.to(d)), y.to(d))
+        loss.backward()
+        out.append((loss.item(), {n: p.grad.double().cpu()
+                                  for n, p in mod.named_parameters()}))
+    assert abs(out[0][0] - out[1][0]) < 1e-4
+    close(*out, 2.0 ** -3 if "keep" in kw else 1e-3)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("kw", KW[:2], ids=str)
+def test_a_model_cast_to_16_bits(dev, kw):
+    """Its masks are 16-bit numbers too, which the fused products do not
+    take."""
+    m = vit(dev, **kw).to(torch.bfloat16)
+    out = m(torch.randn(2, 3, 32, 32, device=dev, dtype=torch.bfloat16))
+    out.float().sum().backward()
+    assert all(p.grad.isfinite().all() for p in m.parameters())
 
 
 @pytest.mark.parametrize("dev", DEVICES)

@@ -16,13 +16,14 @@ Options beyond the reference, off by default, make a block run on the fused
 operators (``Block._fused``), with bias, GELU and residual in the products'
 epilogues: ``fused=True`` is that alone, ``norm="rms"`` takes root-mean-square
 norms that add the residual on the way, ``keep="e4m3"`` holds what the linear
-layers and the MLP's GELU need for the backward pass in 8 bits. They compute in
-16 bits on a GPU: under autocast or with the layers' caches enabled.
+layers and the MLP's GELU need for the backward pass in 8 bits.
 
-The fused operators pass by their modules' calls. A block with a hook on one of
-its modules, a hook on all modules, or another module in place of one of them
-therefore runs module by module, with the same results up to rounding; of what
-it keeps, only the GELU's input is then in 8 bits.
+On a GPU the fused products compute in 16 bits: under autocast or with the
+layers' caches enabled. And they pass by their modules' calls. A block in
+float32 there, with a hook on one of its modules, a hook on all modules, or
+another module in place of one of them therefore runs module by module, with the
+same results up to rounding; of what it keeps, only the GELU's input is then in
+8 bits.
 """
 
 from __future__ import annotations
@@ -162,19 +163,21 @@ class Block(nn.Module):
     def forward(self, x):
         rms = isinstance(self.norm1, FusedRMSNorm)
         if (self.fused or self.keep is not None or rms) \
-                and self._fusible(rms):
+                and self._fusible(x, rms):
             return self._fused(x, rms)
         x = x + self.attn(self.norm1(x))
         x = x + self.mlp(self.norm2(x))
         return x
 
-    def _fusible(self, rms: bool) -> bool:
-        """Whether nothing hangs on the calls that ``_fused`` passes by."""
+    def _fusible(self, x, rms: bool) -> bool:
+        """Whether nothing hangs on the calls that ``_fused`` passes by, and
+        its products compute in the type at hand."""
         a, m = self.attn, self.mlp
         if _has_any_global_hook() or not (_bare(a, Attention.forward)
                                           and _bare(m, Mlp.forward)):
             return False
         return all(_bare(layer, Conv1dMask.forward, LinearMask.forward)
+                   and layer.fusible(x)
                    for layer in (a.qkv, a.proj, m.fc1, m.fc2)) \
             and (not rms or _bare(self.norm1, FusedRMSNorm.forward)
                  and _bare(self.norm2, FusedRMSNorm.forward)) \

@@ -94,6 +94,19 @@ class _MaskedMixin:
             return torch.get_autocast_dtype(x.device.type)
         return self.compute_dtype
 
+    def fusible(self, x: torch.Tensor) -> bool:
+        """Whether ``fused`` takes an ``x`` of this type and device: it masks
+        by float32 values, and on a GPU it computes in 16 bits."""
+        if self.mask.dtype != torch.float32:
+            return False
+        if self.weight_masked is not None:
+            t = self.weight_masked.dtype
+        else:
+            t = self._fused_dtype(x) or (
+                self.weight.dtype if self.weight.dtype != torch.float32
+                else x.dtype)
+        return not x.is_cuda or t in (torch.bfloat16, torch.float16)
+
     def _load_from_state_dict(self, *args, **kwargs):
         super()._load_from_state_dict(*args, **kwargs)
         self.refresh_cache()
