@@ -20,6 +20,7 @@ Device handling honors the model's device (the reference hardcodes
 
 from __future__ import annotations
 
+import contextlib
 from typing import Any, Iterable, List, Optional
 
 import torch
@@ -51,6 +52,21 @@ def _rewrite_masks(model: nn.Module, scores: dict, threshold: float) -> None:
         m.refresh_cache()
 
 
+@contextlib.contextmanager
+def _nothing_in_8_bits(model: nn.Module):
+    """Scores are made of gradients at the activations' own values: what a
+    model keeps in 8 bits for training is not kept so meanwhile."""
+    kept = [(m, m.keep) for m in model.modules()
+            if getattr(m, "keep", None) is not None]
+    for m, _ in kept:
+        m.keep = None
+    try:
+        yield
+    finally:
+        for m, keep in kept:
+            m.keep = keep
+
+
 @torch.no_grad()
 def prune_mag(model: nn.Module, density: float) -> nn.Module:
     """Magnitude pruning: score = |mask * weight|
@@ -77,7 +93,8 @@ def prune_snip(model: nn.Module, density: float,
     inputs = inputs.to(device, non_blocking=True)
     targets = targets.to(device, non_blocking=True)
     use_amp = device.type == "cuda" and amp_dtype != torch.float32
-    with torch.autocast(device_type="cuda", dtype=amp_dtype, enabled=use_amp):
+    with torch.autocast(device_type="cuda", dtype=amp_dtype,
+                        enabled=use_amp), _nothing_in_8_bits(model):
         out = model(inputs)
         loss = TF.cross_entropy(out, targets)
     loss.backward()
@@ -125,7 +142,7 @@ def prune_synflow(model: nn.Module, density: float,
     model.zero_grad(set_to_none=True)
     use_amp = device.type == "cuda" and amp_dtype != torch.float32
     with torch.autocast(device_type="cuda", dtype=amp_dtype,
-                        enabled=use_amp):
+                        enabled=use_amp), _nothing_in_8_bits(model):
         out = model(ones)
         if isinstance(out, tuple):
             out = out[0]
