@@ -198,9 +198,15 @@ def _linear_act_fwd(x, w, bias, residual, act, keep, keep_x):
             *(act8.quantize_act8(x) if keep_x else (None, None)))
 
 
+def _product32(a, b):
+    """In 32 bits, whatever autocast says."""
+    with torch.autocast(a.device.type, enabled=False):
+        return a.float() @ b.float()
+
+
 def _linear_act_fwd_plain(x, w, bias, residual, act, keep):
     from turboprune_amd.ops.norm_act import gelu_plain
-    z = x.float() @ w.float().t()
+    z = _product32(x, w.t())
     if bias is not None:
         z = z + bias.float()
     y = z if act is None else gelu_plain(z)
@@ -225,11 +231,11 @@ def _linear_act_bwd_plain(dy, z, zs, xk, xs, w, mask, want_dx, dw_type, db_type)
         dz = dz * gelu_slope(z)
     dx = dw = db = None
     if want_dx:
-        dx = (dz @ w.float()).to(w.dtype)
+        dx = _product32(dz, w).to(w.dtype)
     if dw_type is not None:
         x = xk.float() if xs is None else \
             act8.dequantize_act8(Act8(xk, xs), torch.float32)
-        dw = dz.t() @ x
+        dw = _product32(dz.t(), x)
         if mask is not None:
             dw = torch.where(mask.reshape(dw.shape) != 0, dw,
                              torch.zeros_like(dw))
