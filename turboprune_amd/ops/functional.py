@@ -354,11 +354,12 @@ def masked_linear_act(x: torch.Tensor, weight: torch.Tensor,
 def _masked_compute(weight, mask, dtype):
     if mask is None:
         return weight.to(dtype)
-    if weight.dtype == torch.float32 and dtype in (torch.float32,
-                                                   torch.bfloat16):
+    if _backend.use_native(weight, mask) and weight.dtype == torch.float32 \
+            and dtype == torch.bfloat16:
         if torch.jit.is_tracing():
             return MaskedWeight.apply(weight, mask, None, dtype)
         return mask_apply(weight, mask, dtype)
+    # chosen, not multiplied: an infinity in a masked place stays there
     return torch.where(mask != 0, weight, torch.zeros_like(weight)).to(dtype)
 
 
