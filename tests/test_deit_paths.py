@@ -139,6 +139,28 @@ def test_a_model_cast_to_16_bits(dev, kw):
     assert all(p.grad.isfinite().all() for p in m.parameters())
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("kw", KW, ids=str)
+def test_half_precision_under_autocast(kw):
+    """float16 products, which the layers' caches do not offer: under autocast
+    without them."""
+    out = []
+    for model in (vit("cuda", **{k: v for k, v in kw.items() if k == "norm"}),
+                  vit("cuda", **kw)):
+        if not out:                    # the first runs module by module
+            for b in model.blocks:
+                b.mlp.register_forward_hook(lambda *a: None)
+        torch.manual_seed(3)
+        x = torch.randn(6, 3, 32, 32).cuda()
+        y = torch.randint(0, 10, (6,)).cuda()
+        with torch.autocast("cuda", torch.float16):
+            loss = nn.functional.cross_entropy(model(x).float(), y)
+        (loss * 1024).backward()       # small gradients stay in the range
+        out.append((loss.item(), {n: p.grad.double().cpu() / 1024
+                                  for n, p in model.named_parameters()}))
+    close(*out, 2.0 ** -3 if "keep" in kw else 2.0 ** -7)
+
+
 @pytest.mark.parametrize("dev", DEVICES)
 def test_codes_only_where_they_are_kept(dev, monkeypatch):
     """The norms write 8-bit rows for the product behind them, which keeps them
