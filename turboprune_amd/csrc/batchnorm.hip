@@ -289,7 +289,7 @@ __global__ void bn_apply_kernel(const T* __restrict__ x,
 // ---------------- backward reduce ----------------------------------------
 // accumulates sum_g = Σ dy_eff and sum_gx = Σ dy_eff * x per channel
 // (the xhat projection Σ g·xhat = rstd·(sum_gx − mean·sum_g) is applied
-// in the finalize kernel — keeps the hot loop at ~3 packed VALU/dword).
+// in the finalize kernel — keeps the hot loop at two sums a value).
 template <typename T, bool RELU>
 __global__ void bn_bwd_reduce_kernel(const T* __restrict__ x,
                                      const uint8_t* __restrict__ rmask,

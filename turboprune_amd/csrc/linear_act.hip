@@ -7,6 +7,11 @@
 //
 // All three products run on one tiled matrix kernel (mm_kernel below), a few
 // rows on one that stages nothing (rows_kernel).
+//
+// Sizes are rows x K -> N throughout, as of the product that a launch computes.
+// Times are of launches after a pause or a few of them; ten large products in a
+// row lower the chip's clock and take up to a fifth longer (25216 x 4096 ->
+// 1024 208 us, then 250).
 
 #include <ATen/ATen.h>
 #include <ATen/hip/HIPContext.h>
@@ -227,9 +232,9 @@ struct CodeTile {
 
 // Q's values of one k-tile, from LDS, in 8 bits. The column tiles of a row of
 // tiles take the k-tiles in turn, so that each of them does its share and the
-// input is read once for product and codes: 50432x384x1536 with a 32-bit
-// residual 144 us, with a pass of its own 42 + 105 and a launch more (342 and
-// 354 us for the layer forward and backward).
+// input is read once for product and codes: 50432 x 1536 -> 384 with a 32-bit
+// residual 144 us, with a pass of its own 42 + 105 and a launch more (332 and
+// 354 us for the layer forward and backward when both were measured).
 template <typename T, int BQ, int BK, int THREADS>
 TP_DEVICE void keep_tile(TP_LDS const char* t, const Mm& a, int m0, int kt) {
   constexpr int C = BK / 8;
@@ -280,11 +285,11 @@ struct LanesMax {   // over lanes l, l^16, l^32, l^48
   }
 };
 
-// When a k-tile's successor is fetched: behind the reads of the first
-// fragments (the waves' first products then do not wait behind address
-// arithmetic: 131 -> 120 us for 50432x1536x384 with GELU and codes), behind
-// those of all, or between the two halves of the products. Which is best goes
-// by the registers that are left: all fragments of 16 waves at once spill.
+// When a k-tile's successor is fetched: behind the reads of the first fragments
+// (the waves' first products then do not wait behind address arithmetic: 131 ->
+// 120 us for 50432 x 384 -> 1536 with GELU and codes), behind those of all, or
+// between the two halves of the products. Which is best goes by the registers
+// that are left: all fragments of 16 waves at once spill.
 enum { kAfterFirst = 0, kAfterReads = 1, kBetween = 2 };
 
 // What follows the sum: nothing but the residual, GELU with z kept in 16 bits
@@ -379,11 +384,11 @@ TP_DEVICE void epilogue8(const Epi& e, int64_t at, int64_t blk, int n,
 // C = Q P, a tile to a block: BK values of the sum at a time go into LDS by
 // asynchronous 16-byte loads, a step ahead of the one that is multiplied, with
 // one barrier a step; WQ x WP waves share the tile, their sums in registers
-// until the epilogue. 25216x1024x4096 in 256 x 256 takes 200 us (1060 TF/s):
-// 1.6 us for a step of 64, which is what a library product of 8192 x 8192 x
-// 8192 takes for as much (1370 TF/s), but 396 tiles occupy 256 CUs twice.
-// Tried without gain: three and four stages of 32 (a barrier costs more than
-// the longer lead gives), fragments of the next half read ahead of the
+// until the epilogue. 25216 x 4096 -> 1024 in 256 x 256 takes 200 us (1060
+// TF/s): 1.6 us for a step of 64, which is what a library product of 8192 x
+// 8192 x 8192 takes for as much (1370 TF/s), but 396 tiles occupy 256 CUs
+// twice. Tried without gain: three and four stages of 32 (a barrier costs more
+// than the longer lead gives), fragments of the next half read ahead of the
 // products, lines brought into L2 two and three steps ahead, steps begun at
 // another place in every block.
 template <typename T, int BQ, int BP, int BK, int WQ, int WP, int QF, int PF,
@@ -543,18 +548,19 @@ __global__ __launch_bounds__(WQ * WP * 64, MINW) void mm_kernel(Mm a) {
 }
 
 // Few rows (single tokens, one image, a classifier's batch): nothing is used
-// often enough for tiles to pay, and the staged kernel would give 29x2875x768
-// to 12 CUs, each waiting for 45 loads in turn. A block takes 32 columns and
-// MI x 16 rows; its 8 waves take 32 values of k each in turn, straight from
+// often enough for tiles to pay, and the staged kernel would give 29 x 2875 ->
+// 768 to 12 CUs, each waiting for 45 loads in turn. A block takes 32 columns
+// and MI x 16 rows; its 8 waves take 32 values of k each in turn, straight from
 // global memory into fragments (rows at any address), and their sums meet in
 // LDS, wave j finishing 16 rows. Bound by the latency of the few steps that
-// each wave makes (1x384x1000 and 1x768x768 3.7 and 4.3 us), then by what a
-// block reads: 1x4096x4096 13 us, 2.6 TB/s, weights from memory.
+// each wave makes (1 x 384 -> 1000 and 1 x 768 -> 768 4 us), then by what a
+// block reads: 1 x 4096 -> 4096 13 us, 2.6 TB/s, weights from memory.
 //
 // 8 values of a row from p on. Where rows have an odd length they start between
 // two dwords every other time, and a 16-byte load there is taken apart by the
 // memory pipe: such lanes load the five dwords around their values and shift
-// (29x2875x768: 17 us, 27 with loads at odd addresses; 12 where K is even).
+// (29 x 2875 -> 768: 17 us, 27 with loads at odd addresses; 12 where K is
+// even).
 template <typename T, bool ODD>
 struct Few {
   u32x4 d;
@@ -790,12 +796,13 @@ __global__ __launch_bounds__(kBlock) void turn_kernel(Turn a) {
 
 // dz = dy act'(z), rounded to the products' 16 bits (matrix instructions take
 // no more of them at that rate; it adds as much to a gradient's error as the
-// rounding of the gradient itself), and the column sums of dz, unrounded. 32
-// threads take 256 neighbouring columns, 8 rows at a time; a block adds its
-// rows in registers and joins them in LDS, so the sums need no atomics and keep
-// their order. Bound by memory: 50432 x 1536 with z in 8 bits 84 us, 4.6 TB/s.
-// The blocks behind the rows' turn the weight over meanwhile, which takes 5 us
-// by itself, of latency.
+// rounding of the gradient itself, and in fp16 it has that type's range: what
+// overflows arrives as an infinity, by which a gradient scaler finds it), and
+// the column sums of dz, unrounded. 32 threads take 256 neighbouring columns, 8
+// rows at a time; a block adds its rows in registers and joins them in LDS, so
+// the sums need no atomics and keep their order. Bound by memory: 50432 x 1536
+// with z in 8 bits 84 us, 4.6 TB/s. The blocks behind the rows' turn the weight
+// over meanwhile, which takes 5 us by itself, of latency.
 struct Dz {
   const void* dy;
   const void* z;           // 16-bit values or codes; null without act
@@ -955,13 +962,13 @@ int64_t tiles_of(const Mm& a, int q, int p) {
 
 // Groups of 16 rows that a block of rows_kernel takes, 0: the tiles. Such
 // blocks hold little and read much, so they win while the chip has a CU for
-// each, and the smallest that still have one win most (fp16, us, with 1, 2
-// and 4 groups to a block, and the staged kernel in 64 x 64): 64x4096x1024
-// 13.4, 16.8, 23.7, 32.6; 197x768x768 6.7, 5.6, 6.9, 7.3; 128x4096x4096 (128
-// column blocks, so 4 groups) 47, 32, 25, 34. Past that many blocks the tiles
-// win, 197x1024x4096 in 11.6 against 14.7, but for a weight that is read once
-// all the same: 16x1024x16384 8.2 against 11.5, 32 rows 10.0 against 11.6, 64
-// rows 15.2 against 11.6.
+// each, and the smallest that still have one win most (fp16, us, with 1, 2 and
+// 4 groups to a block, and the staged kernel in 64 x 64): 64 x 4096 -> 1024
+// 13.4, 16.8, 23.7, 32.6; 197 x 768 -> 768 6.7, 5.6, 6.9, 7.3; 128 x 4096 ->
+// 4096 (128 column blocks, so 4 groups) 47, 32, 25, 34. Past that many blocks
+// the tiles win, 197 x 1024 -> 4096 in 11.6 against 14.7, but for a weight that
+// is read once all the same: 16 x 1024 -> 16384 8.2 against 11.5, 32 rows 10.0
+// against 11.6, 64 rows 15.2 against 11.6.
 int row_groups(int64_t M, int64_t N) {
   int64_t cols = (N + 31) / 32;
   for (int g = 1; g <= 4; g *= 2)
@@ -989,8 +996,8 @@ void run_few(const Mm& a, int groups) {
 }
 
 // Both operands along the sum. Short products end soonest in many small tiles:
-// 1576x768x768 10.2 us in 64 x 64, 12.0 in 128 x 128; 3152x1536x384 (1200
-// small tiles) 13.8 against 12.9.
+// 1576 x 768 -> 768 10.2 us in 64 x 64, 12.0 in 128 x 128; 3152 x 384 -> 1536
+// (1200 small tiles) 13.8 against 12.9.
 //
 // Of the large tiles 256 x 256 by 16 waves moves the fewest bytes into LDS per
 // product, but a CU holds one, and one tile more than CUs doubles the time. Of
@@ -1002,11 +1009,11 @@ void run_few(const Mm& a, int groups) {
 // and without a 32-bit residual) this finds the fastest within 1 % on average
 // and 14 % at most; 256 x 256 wherever it is well filled, else 128 x 128, is
 // 7 % and 47 % off. In us, 256 x 256, 160 x 128, 128 x 128:
-//   50432x1536x384, GELU, codes   118  135  137
-//   50432x384x1536, residual      126   99  110
-//   25216x1024x4096               199  211  225
-//   25216x768x2560                120   94  108
-//   6304x1024x4096                 85   76   63
+//   50432 x 384 -> 1536, GELU, codes   118  135  137
+//   50432 x 1536 -> 384, residual      126   99  110
+//   25216 x 4096 -> 1024               199  211  225
+//   25216 x 2560 -> 768                120   94  108
+//   6304 x 4096 -> 1024                 85   76   63
 std::tuple<int64_t, int64_t> rows_tile(int64_t M, int64_t N) {
   if (tiles_of(M, N, 64, 64) <= 600) return {64, 64};
   auto cost = [&](int q, int p, int one) {
@@ -1037,12 +1044,15 @@ void run_rows(const Mm& a) {
   }
 }
 
-// Both across the sum (weight gradients), in slabs of it: as many as fill the
-// chip, none shorter than four k-tiles. 4096x1024 over 25216 rows takes 197 us
-// in 256 x 256 tiles and 235 in 128 x 128; 1536x384 over 50432 rows 88 us in
-// 128 x 128 and 95 in 256 x 256, whose third column tile is half empty.
-// Codes go through registers, which 16 waves leave too few of: 8 waves there
-// (200 us against 285; 128 x 128 266).
+// Both across the sum (weight gradients), in slabs of it: as many as go into
+// one round of the chip (256 blocks, 512 of the smaller tiles), none shorter
+// than four k-tiles. Rounds are not counted, so a weight of just over half a
+// round's tiles (129 of 256) has one slab and leaves the other CUs idle. A
+// gradient of 4096 x 1024 over 25216 rows takes 197 us in 256 x 256 tiles and
+// 235 in 128 x 128; 1536 x 384 over 50432 rows 88 us in 128 x 128 and 95 in 256
+// x 256, whose third column tile is half empty. Codes go through registers,
+// which 16 waves leave too few of: 8 waves there (200 us against 285; 128 x 128
+// 266).
 struct Split {
   int tile, slabs;
 };
@@ -1195,7 +1205,8 @@ linear_act_bwd(const at::Tensor& dy_in, const c10::optional<at::Tensor>& z,
                const c10::optional<at::Tensor>& zscale,
                const c10::optional<at::Tensor>& xkept,
                const c10::optional<at::Tensor>& xscale, const at::Tensor& w,
-               const c10::optional<at::Tensor>& mask, bool want_dx, c10::optional<at::ScalarType> dw_type,
+               const c10::optional<at::Tensor>& mask, bool want_dx,
+               c10::optional<at::ScalarType> dw_type,
                c10::optional<at::ScalarType> db_type) {
   TORCH_CHECK(dy_in.is_cuda() && dy_in.dim() == 2 && w.dim() == 2 &&
                   is16(w.scalar_type()) && dy_in.device() == w.device() &&
@@ -1219,9 +1230,9 @@ linear_act_bwd(const at::Tensor& dy_in, const c10::optional<at::Tensor>& z,
   bool products = want_dx || dw_type.has_value();
   at::Tensor dz = same ? dy : at::empty({products ? M : 0, ldz}, opt), part;
   c10::optional<at::Tensor> dx, dw, db;
-  // w along the sum: turned over first where the product is long enough to
-  // win it back (50432x384x1536 in 128 x 128: 95 us and 5 for the turn, 111
-  // across; 25216x1024x4096: 214 and 6, 282 across)
+  // w along the sum: turned over first where the product is long enough to win
+  // it back (50432 x 1536 -> 384 in 128 x 128: 95 us and 5 for the turn, 111
+  // across; 25216 x 4096 -> 1024: 214 and 6, 282 across)
   Mm in{};
   in.M = (int)M;
   in.N = (int)K;

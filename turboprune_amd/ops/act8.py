@@ -8,9 +8,10 @@ most 2^-4 of itself (half a step of e4m3), or by 2^-10 of its block's scale
 where it is that small. NaN and infinities become NaN. 1.03 bytes a value,
 against 2 in bfloat16.
 
-Dequantised values are exact in bfloat16, so the matrix products of a
-backward pass that reads them (``functional.masked_linear_act``) add nothing
-to the error of keeping.
+Dequantised values are exact in bfloat16, so reading them as such for the matrix
+products of a backward pass (``functional.masked_linear_act``) adds nothing to
+the error of keeping. What those products add is the rounding of the gradient
+that they multiply them by to the compute type.
 
 CPU tensors take the plain PyTorch form below, which is also the kernels'
 numerics oracle.

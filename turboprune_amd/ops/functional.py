@@ -263,14 +263,21 @@ def masked_linear_act(x: torch.Tensor, weight: torch.Tensor,
     or ``"gelu"`` (exact). ``cache`` and ``compute_dtype`` are
     ``masked_linear``'s: the masked weight in the compute type, and that type
     where there is no cache. The compute type is bfloat16 or float16 on a GPU
-    (also float32 on the CPU); an ``x`` of another type is cast to it.
+    (also float32 on the CPU); an ``x`` of another type is cast to it. For
+    float32 products on a GPU there is ``masked_linear``: the matrix
+    instructions that this kernel is made of take 16-bit operands. At most 2^30
+    rows, and 2^20 values in a row of ``x`` and of the output.
 
     For the backward pass the input and, with an activation, the
     pre-activation are kept: in the compute type, or with ``keep="e4m3"`` in
     the 8-bit format of ``ops.act8`` (the gradients are then taken at the
     values it stands for). ``kept`` is ``x`` already in that format, as
     ``add_rms_norm`` hands it on. The weight's gradient is masked and has the
-    weight's type.
+    weight's type. The gradient of the pre-activation is rounded to the compute
+    type (on a GPU) before the products that give ``x``'s and the weight's, as
+    between two layers of that type; the bias's is summed before that rounding.
+    Sums are in 32 bits, in an order that does not change from call to call.
+    Neither gradients of gradients nor, on a GPU, forward-mode derivatives.
     """
     native = _backend.use_native(x)
     tracing = torch.jit.is_tracing()

@@ -202,7 +202,8 @@ class LinearMask(_MaskedMixin, nn.Linear):
               kept=None) -> torch.Tensor:
         """``act(forward(x)) + residual`` in one product with an epilogue
         (``functional.masked_linear_act``); ``keep="e4m3"`` holds what the
-        backward pass needs in 8 bits."""
+        backward pass needs in 8 bits. A method beside ``forward``: the
+        module's hooks do not run."""
         return TF.masked_linear_act(
             x, self.weight, self.mask, self.bias, residual, act,
             self._fresh_cache(), self._fused_dtype(x), keep, kept)

@@ -225,7 +225,8 @@ def add_rms_norm(x: torch.Tensor, residual: Optional[torch.Tensor],
     its type or float32; ``out_dtype`` is ``x``'s type, or a 16-bit type where
     ``x`` is float32; ``weight`` is a vector of the last dimension's length
     in any of the three types. Rows may lie at any distance. Statistics and
-    the weight's gradient are summed in float32, in a fixed order.
+    the weight's gradient are summed in float32, in a fixed order. Neither
+    gradients of gradients nor, on a GPU, forward-mode derivatives.
     """
     native = _backend.use_native(x)
     if native and not torch.jit.is_tracing():
