@@ -7,8 +7,6 @@ import torch
 
 from test_linear_act import BF16, F32, FP16, check, make
 
-pytestmark = pytest.mark.gpu
-
 SIZES = {(64, 64): [(300, 72, 200), (1025, 100, 1001)],
          (128, 128): [(5000, 136, 500)],
          (160, 128): [(9000, 200, 500), (12608, 72, 383)],
@@ -20,12 +18,14 @@ def tile(M, N):
     return tuple(extension().linear_act_tile(M, N))
 
 
+@pytest.mark.gpu
 def test_sizes_reach_their_tiles():
     for want, sizes in SIZES.items():
         for M, _, N in sizes:
             assert tile(M, N) == want
 
 
+@pytest.mark.gpu
 @pytest.mark.parametrize("M,K,N", [s for v in SIZES.values() for s in v])
 @pytest.mark.parametrize("keep", [None, "e4m3"])
 @pytest.mark.parametrize("res", [None, BF16, F32])
@@ -33,6 +33,7 @@ def test_gelu(M, K, N, keep, res):
     check(make(M, K, N, BF16, res, "cuda"), BF16, "gelu", keep)
 
 
+@pytest.mark.gpu
 @pytest.mark.parametrize("M,K,N", [v[-1] for v in SIZES.values()])
 @pytest.mark.parametrize("res", [None, FP16, F32])
 def test_half_and_without_activation(M, K, N, res):
@@ -47,6 +48,7 @@ WEIGHTS = {(64, False): [(60, 130, 70)], (64, True): [(900, 72, 200)],
            (256, False): [(200, 2050, 2300)], (256, True): [(5000, 1000, 1001)]}
 
 
+@pytest.mark.gpu
 def test_weights_reach_their_tiles():
     from turboprune_amd.ops._backend import extension
     for (want, split), sizes in WEIGHTS.items():
@@ -55,6 +57,7 @@ def test_weights_reach_their_tiles():
             assert (t, slabs > 1) == (want, split), (M, K, N, t, slabs)
 
 
+@pytest.mark.gpu
 @pytest.mark.parametrize("M,K,N", [s for v in WEIGHTS.values() for s in v])
 @pytest.mark.parametrize("t", [BF16, FP16])
 @pytest.mark.parametrize("keep", [None, "e4m3"])
@@ -62,3 +65,18 @@ def test_weights_reach_their_tiles():
 def test_weight_gradients(M, K, N, t, keep, weight):
     check(make(M, K, N, t, None, "cuda",
                weight=t if weight == "same" else F32), t, None, keep)
+
+
+def test_sizes_of_nothing_are_refused():
+    from turboprune_amd.ops import _backend
+    if not _backend.has_extension():
+        pytest.skip("needs the extension, but no GPU")
+    ext = _backend.extension()
+    for bad in (lambda: ext.linear_act_tile(0, 64),
+                lambda: ext.linear_act_tile(64, -1),
+                lambda: ext.linear_act_tile(1 << 40, 64),
+                lambda: ext.linear_act_split(0, 64, 64),
+                lambda: ext.linear_act_split(64, 0, 64),
+                lambda: ext.linear_act_split(64, 64, 1 << 21)):
+        with pytest.raises(RuntimeError):
+            bad()

@@ -1094,11 +1094,14 @@ void check_size(int64_t M, int64_t N, int64_t K) {
 // rows and columns of the tiles that a product of M x N values along both rows
 // runs in (few rows without a gradient aside)
 std::tuple<int64_t, int64_t> linear_act_tile(int64_t M, int64_t N) {
+  TORCH_CHECK(M > 0 && N > 0, "linear_act_tile: sizes from 1 on");
+  check_size(M, N, 1);
   return rows_tile(M, N);
 }
 // rows and columns of the tiles, and slabs, of the gradient of an N x K weight
 // over M rows
 std::tuple<int64_t, int64_t> linear_act_split(int64_t M, int64_t N, int64_t K) {
+  TORCH_CHECK(M > 0 && N > 0 && K > 0, "linear_act_split: sizes from 1 on");
   check_size(M, N, K);
   Mm a{};
   a.M = (int)N;
