@@ -31,3 +31,16 @@ def test_an_error_leaves_the_model_as_it_was():
                              torch.randint(0, 10, (8,)))])
     assert all(b.keep == "e4m3" and b.mlp.act.keep == "e4m3"
                for b in m.blocks)
+
+
+def test_other_modules_keep_is_their_own():
+    class Scale(torch.nn.Module):
+        keep = 0.5
+
+        def forward(self, x):
+            return x * self.keep
+    m = vit("cpu", keep="e4m3")
+    m.blocks.append(Scale())
+    prune_snip(m, 0.3, [(torch.randn(8, 3, 32, 32),
+                         torch.randint(0, 10, (8,)))])
+    assert m.blocks[2].keep == 0.5

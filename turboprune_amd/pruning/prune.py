@@ -26,8 +26,10 @@ from typing import Any, Iterable, List, Optional
 import torch
 import torch.nn as nn
 
+from turboprune_amd.models.deit import Block
 from turboprune_amd.ops import functional as TF
 from turboprune_amd.ops.mask_layers import masked_modules
+from turboprune_amd.ops.norm_act import FusedGELU
 
 
 def _model_device(model: nn.Module) -> torch.device:
@@ -56,14 +58,14 @@ def _rewrite_masks(model: nn.Module, scores: dict, threshold: float) -> None:
 def _nothing_in_8_bits(model: nn.Module):
     """Scores are made of gradients at the activations' own values: what a
     model keeps in 8 bits for training is not kept so meanwhile."""
-    kept = [(m, m.keep) for m in model.modules()
-            if getattr(m, "keep", None) is not None]
-    for m, _ in kept:
+    kept = [m for m in model.modules() if isinstance(m, (Block, FusedGELU))]
+    was = [m.keep for m in kept]
+    for m in kept:
         m.keep = None
     try:
         yield
     finally:
-        for m, keep in kept:
+        for m, keep in zip(kept, was):
             m.keep = keep
 
 
