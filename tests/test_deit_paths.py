@@ -109,6 +109,18 @@ def test_replaced_modules(dev, kw):
 
 
 @pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.filterwarnings("ignore")
+def test_a_recorded_module_in_place(dev):
+    """One that torch.jit.trace made has no forward method on its class."""
+    m = vit(dev, norm="rms")
+    mlp = nn.Sequential(nn.Linear(96, 96), nn.Tanh()).to(dev)
+    m.blocks[0].mlp = torch.jit.trace(mlp, torch.randn(2, 17, 96, device=dev))
+    ref = vit(dev, norm="rms")
+    ref.blocks[0].mlp = mlp
+    close(step(ref, dev), step(m, dev), 2.0 ** -5)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
 @pytest.mark.parametrize("kw", KW, ids=str)
 def test_float32_training(dev, kw):
     """Without autocast and caches the products are float32, which the fused

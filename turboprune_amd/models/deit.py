@@ -142,9 +142,10 @@ def _bare(module: nn.Module, *forwards) -> bool:
     """Whether a call of the module runs one of these methods and nothing
     else."""
     d = module.__dict__
-    return type(module).forward in forwards and "forward" not in d and not (
-        d["_forward_hooks"] or d["_forward_pre_hooks"]
-        or d["_backward_hooks"] or d["_backward_pre_hooks"])
+    return getattr(type(module), "forward", None) in forwards \
+        and "forward" not in d and not (
+            d["_forward_hooks"] or d["_forward_pre_hooks"]
+            or d["_backward_hooks"] or d["_backward_pre_hooks"])
 
 
 class Block(nn.Module):
